@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define SONIC_B200_ABI_VERSION 4
+#define SONIC_B200_ABI_VERSION 5
 
 /* Candidate-set width of the two-stage top-k (reference ops/base.py:24, MAX_K). */
 #define SONIC_MAX_K 128
@@ -59,7 +59,9 @@ enum {
   SONIC_DTYPE_BF16 = 0,
   SONIC_DTYPE_F32 = 1,
   SONIC_DTYPE_I32 = 2,
-  SONIC_DTYPE_I64 = 3
+  SONIC_DTYPE_I64 = 3,
+  SONIC_DTYPE_F16 = 4,
+  SONIC_DTYPE_E4M3 = 5   /* 8-bit float, 3 mantissa bits, finite (largest value 448) */
 };
 
 /* Call flags (bit set in the `flags` field of each argument struct). */
@@ -81,7 +83,11 @@ enum {
   /* A bounded wait for a bulk copy into shared memory gave up. The rows (singular, top-k) or
    * requests (multistep) of the affected CTAs wrote none of their outputs; the staged noise
    * rows of sonic_indexed_copy that timed out were not stored. */
-  SONIC_DEVICE_ERR_WAIT = 1u << 0
+  SONIC_DEVICE_ERR_WAIT = 1u << 0,
+  /* A page id outside the cache, or a sequence length outside its page-table row. Nothing outside
+   * the cache was read or written: the token's write was skipped, its read-back gave zeros, and
+   * the attention of that request is unspecified. */
+  SONIC_DEVICE_ERR_PAGE = 1u << 1
 };
 
 /*
@@ -281,7 +287,8 @@ sonic_status sonic_fused_singular_static(const SonicSingularArgs* args, void* st
 
 /* Reads the device error word (SONIC_DEVICE_ERR_* bits, 0 when clean) that the kernels of
  * earlier calls left in `workspace` (the buffer passed as args->workspace to
- * sonic_fused_singular, sonic_fused_multistep, sonic_bounded_topk or sonic_shard_candidates)
+ * sonic_fused_singular, sonic_fused_multistep, sonic_bounded_topk, sonic_shard_candidates or
+ * sonic_paged_attention, or the word passed as `error` to sonic_cache_append / _gather)
  * into *error_out, then clears it. With workspace == NULL it reads the library's own word on the
  * current device, which sonic_fused_singular_static and sonic_indexed_copy write. The word
  * stays set across calls until read. Synchronises `stream`: do not call it while the stream
@@ -381,6 +388,142 @@ typedef struct SonicPopulateArgs {
  * inputs (prompt tokens, bias entries). Noise refresh stays with the caller's generator.
  * Runs on `stream`, allocates nothing, never synchronises. */
 sonic_status sonic_populate_slots(const SonicPopulateArgs* args, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Decode-side operators: the paged key-value cache, the attention of new tokens over it, and the
+ * residual norm. No counterpart in the reference: they are what a served model runs between the
+ * sampler's calls. The accepted counts of sonic_fused_multistep move `lengths` on the device, so a
+ * rejected draft needs no write to the cache: its rows lie past the new length.
+ * ------------------------------------------------------------------------------------- */
+
+/*
+ * A paged cache of one layer. Token slot s of page p holds, for kv head h, the head_dim keys at
+ * keys + p * page_stride + h * head_stride + s * slot_stride (elements; the values likewise, with
+ * the same strides). Rows start on 16-byte boundaries. dtype is bf16, f16, or e4m3 with one fp32
+ * scale per (token, head) at key_scales + p * scale_page_stride + h * scale_head_stride + s: a
+ * row stands for code * scale.
+ */
+typedef struct SonicPagedCache {
+  void* keys;
+  void* values;
+  float* key_scales;         /* e4m3 only, else NULL */
+  float* value_scales;
+  int32_t dtype;             /* SONIC_DTYPE_BF16 / _F16 / _E4M3 */
+  int32_t pages;
+  int32_t page_size;         /* token slots a page, >= 1 */
+  int32_t kv_heads;
+  int32_t head_dim;          /* 64, 128 or 256 */
+  int64_t page_stride;
+  int64_t head_stride;
+  int64_t slot_stride;
+  int64_t scale_page_stride;
+  int64_t scale_head_stride;
+} SonicPagedCache;
+
+/*
+ * Which tokens a call is about. Request b has lengths[b] tokens in the cache, the call's new ones
+ * included: these are its last n_b, rows [cu_seqlens[b], cu_seqlens[b + 1]) of the call's token
+ * tensors (without cu_seqlens, tokens / requests rows each). The token at position t lies in page
+ * page_table[b * table_stride + t / page_size], slot t % page_size. All arrays are read on the
+ * device, so a captured graph follows them.
+ */
+typedef struct SonicSequences {
+  int32_t requests;
+  int32_t tokens;            /* rows of the call's token tensors */
+  const int32_t* page_table; /* [requests, table_stride] */
+  int64_t table_stride;
+  int32_t table_width;       /* pages a row can hold; lengths beyond it are cut and reported */
+  const int32_t* lengths;    /* [requests] */
+  const int32_t* cu_seqlens; /* [requests + 1] or NULL */
+} SonicSequences;
+
+/* New keys and values into their pages. An e4m3 row x gets the scale c / 448 with
+ * c = max(amax|x|, 2^-60) and the codes e4m3(x * (448 / c)), to nearest even; a NaN or an infinity
+ * makes its row NaN when read back. New tokens at negative positions (lengths[b] < n_b) are
+ * skipped. Two tokens of one call must not share a slot. */
+typedef struct SonicCacheAppendArgs {
+  SonicPagedCache cache;
+  SonicSequences sequences;
+  uint32_t flags;            /* SONIC_FLAG_PDL */
+  int32_t dtype;             /* of keys and values: bf16 or f16; the cache's own, or any with e4m3 */
+  const void* keys;          /* [tokens, kv_heads, head_dim], unit inner stride */
+  const void* values;
+  int64_t key_token_stride;  /* elements; rows start on 16-byte boundaries */
+  int64_t key_head_stride;
+  int64_t value_token_stride;
+  int64_t value_head_stride;
+  uint32_t* error;           /* device error word (SONIC_DEVICE_ERR_PAGE is ORed in) or NULL */
+} SonicCacheAppendArgs;
+
+/* Reading back: the tokens at positions [0, starts[b + 1] - starts[b]) of each request, row
+ * starts[b] + t of the outputs; e4m3 rows as code * scale, rounded once. sequences.lengths and
+ * .cu_seqlens are not read; sequences.tokens is the number of output rows. Rows outside every
+ * request are zero. */
+typedef struct SonicCacheGatherArgs {
+  SonicPagedCache cache;
+  SonicSequences sequences;
+  uint32_t flags;            /* SONIC_FLAG_PDL */
+  int32_t dtype;             /* of the outputs: bf16 or f16; the cache's own, or any with e4m3 */
+  const int32_t* starts;     /* [requests + 1] output rows */
+  void* keys;                /* out [tokens, kv_heads, head_dim], contiguous */
+  void* values;
+  uint32_t* error;
+} SonicCacheGatherArgs;
+
+/* Attention of the call's tokens over their requests' cached keys and values, which already hold
+ * the tokens themselves. Query i of request b stands at position lengths[b] - n_b + i and sees the
+ * keys up to it, the last `window` of them when window > 0. out = sum_j softmax_j(scale q.k_j) v_j,
+ * lse = log sum_j exp(scale q.k_j); a query that sees no key gives 0 and -infinity. What lies at
+ * positions a query does not see never reaches its output, NaN and infinities included. */
+typedef struct SonicPagedAttentionArgs {
+  SonicPagedCache cache;
+  SonicSequences sequences;
+  uint32_t flags;            /* SONIC_FLAG_PDL */
+  int32_t dtype;             /* of queries and out: bf16 or f16 (the cache's own unless it is e4m3) */
+  int32_t q_heads;           /* a multiple of kv_heads; query head h reads kv head h / (q_heads / kv_heads) */
+  int32_t max_tokens;        /* most new tokens a request has, or 0 when unknown: picks a tile height */
+  int32_t window;            /* keys a query sees at most, or 0 for all */
+  float scale;
+  const void* queries;       /* [tokens, q_heads, head_dim], unit inner stride */
+  int64_t q_token_stride;    /* elements; rows start on 16-byte boundaries */
+  int64_t q_head_stride;
+  void* out;                 /* [tokens, q_heads, head_dim], unit inner stride */
+  int64_t out_token_stride;  /* rows start on 8-byte boundaries */
+  int64_t out_head_stride;
+  float* lse;                /* out [tokens, q_heads] contiguous, or NULL */
+  void* workspace;           /* device scratch, zero-filled before first use */
+  size_t workspace_bytes;
+} SonicPagedAttentionArgs;
+
+/* r = x + residual (x alone without one) in fp32, y = r / sqrt(mean(r^2) + eps) * weight.
+ * out gets y, or its e4m3 codes with a scale per row (group 0) or per 128 columns (group 128),
+ * quantised as a cache row is. residual_out gets r rounded to dtype; it may be x or residual. */
+typedef struct SonicResidualNormArgs {
+  int32_t rows;
+  int32_t hidden;            /* 1 to 32768 */
+  int32_t dtype;             /* of x, residual, weight and residual_out: bf16, f16 or f32 */
+  int32_t out_dtype;         /* dtype or e4m3 */
+  int32_t group;             /* e4m3: 0 or 128 */
+  uint32_t flags;            /* SONIC_FLAG_PDL */
+  float eps;
+  const void* x;             /* [rows, x_stride] */
+  int64_t x_stride;
+  const void* residual;      /* [rows, residual_stride] or NULL */
+  int64_t residual_stride;
+  const void* weight;        /* [hidden] */
+  void* out;                 /* [rows, out_stride] */
+  int64_t out_stride;
+  float* scales;             /* e4m3: [rows, groups] contiguous, groups = 1 or ceil(hidden / 128) */
+  void* residual_out;        /* [rows, residual_out_stride] or NULL */
+  int64_t residual_out_stride;
+} SonicResidualNormArgs;
+
+size_t sonic_paged_attention_workspace_size(const SonicPagedAttentionArgs* args);
+
+sonic_status sonic_cache_append(const SonicCacheAppendArgs* args, void* stream);
+sonic_status sonic_cache_gather(const SonicCacheGatherArgs* args, void* stream);
+sonic_status sonic_paged_attention(const SonicPagedAttentionArgs* args, void* stream);
+sonic_status sonic_residual_norm(const SonicResidualNormArgs* args, void* stream);
 
 /* ABI version (SONIC_B200_ABI_VERSION) the library was built with. */
 int32_t sonic_abi_version(void);

@@ -12,7 +12,7 @@ import ctypes
 import os
 from pathlib import Path
 
-ABI_VERSION = 4
+ABI_VERSION = 5
 MAX_K = 128
 MAX_LOOKAHEAD = 15
 
@@ -28,6 +28,8 @@ DT_BF16 = 0
 DT_F32 = 1
 DT_I32 = 2
 DT_I64 = 3
+DT_F16 = 4
+DT_E4M3 = 5
 
 # call flags
 FLAG_PDL = 1 << 0
@@ -41,6 +43,7 @@ FLAG_DEBUG_STALL_RING = 1 << 15
 
 # bits of a workspace's device error word (sonic_workspace_error)
 DEVICE_ERR_WAIT = 1 << 0
+DEVICE_ERR_PAGE = 1 << 1
 
 # parts of sonic_populate_slots
 POPULATE_SCALARS = 0x1
@@ -222,6 +225,110 @@ class PopulateArgs(ctypes.Structure):
     ]
 
 
+class PagedCacheStruct(ctypes.Structure):
+    _fields_ = [
+        ("keys", _vp),
+        ("values", _vp),
+        ("key_scales", _vp),
+        ("value_scales", _vp),
+        ("dtype", _i32),
+        ("pages", _i32),
+        ("page_size", _i32),
+        ("kv_heads", _i32),
+        ("head_dim", _i32),
+        ("page_stride", _i64),
+        ("head_stride", _i64),
+        ("slot_stride", _i64),
+        ("scale_page_stride", _i64),
+        ("scale_head_stride", _i64),
+    ]
+
+
+class SequencesStruct(ctypes.Structure):
+    _fields_ = [
+        ("requests", _i32),
+        ("tokens", _i32),
+        ("page_table", _vp),
+        ("table_stride", _i64),
+        ("table_width", _i32),
+        ("lengths", _vp),
+        ("cu_seqlens", _vp),
+    ]
+
+
+class CacheAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCacheStruct),
+        ("sequences", SequencesStruct),
+        ("flags", _u32),
+        ("dtype", _i32),
+        ("keys", _vp),
+        ("values", _vp),
+        ("key_token_stride", _i64),
+        ("key_head_stride", _i64),
+        ("value_token_stride", _i64),
+        ("value_head_stride", _i64),
+        ("error", _vp),
+    ]
+
+
+class CacheGatherArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCacheStruct),
+        ("sequences", SequencesStruct),
+        ("flags", _u32),
+        ("dtype", _i32),
+        ("starts", _vp),
+        ("keys", _vp),
+        ("values", _vp),
+        ("error", _vp),
+    ]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedCacheStruct),
+        ("sequences", SequencesStruct),
+        ("flags", _u32),
+        ("dtype", _i32),
+        ("q_heads", _i32),
+        ("max_tokens", _i32),
+        ("window", _i32),
+        ("scale", ctypes.c_float),
+        ("queries", _vp),
+        ("q_token_stride", _i64),
+        ("q_head_stride", _i64),
+        ("out", _vp),
+        ("out_token_stride", _i64),
+        ("out_head_stride", _i64),
+        ("lse", _vp),
+        ("workspace", _vp),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class ResidualNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i32),
+        ("hidden", _i32),
+        ("dtype", _i32),
+        ("out_dtype", _i32),
+        ("group", _i32),
+        ("flags", _u32),
+        ("eps", ctypes.c_float),
+        ("x", _vp),
+        ("x_stride", _i64),
+        ("residual", _vp),
+        ("residual_stride", _i64),
+        ("weight", _vp),
+        ("out", _vp),
+        ("out_stride", _i64),
+        ("scales", _vp),
+        ("residual_out", _vp),
+        ("residual_out_stride", _i64),
+    ]
+
+
 #: every symbol include/sonic_b200.h declares
 EXPORTED_SYMBOLS = (
     "sonic_fused_singular_workspace_size",
@@ -236,6 +343,11 @@ EXPORTED_SYMBOLS = (
     "sonic_merge_candidates",
     "sonic_indexed_copy",
     "sonic_populate_slots",
+    "sonic_paged_attention_workspace_size",
+    "sonic_cache_append",
+    "sonic_cache_gather",
+    "sonic_paged_attention",
+    "sonic_residual_norm",
     "sonic_abi_version",
     "sonic_last_error",
 )
@@ -249,6 +361,7 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
         ("sonic_fused_singular_workspace_size", SingularArgs),
         ("sonic_fused_multistep_workspace_size", MultistepArgs),
         ("sonic_bounded_topk_workspace_size", TopKArgs),
+        ("sonic_paged_attention_workspace_size", PagedAttentionArgs),
     ):
         fn = getattr(lib, name)
         fn.argtypes = [ctypes.POINTER(argt)]
@@ -258,6 +371,10 @@ def _declare(lib: ctypes.CDLL) -> ctypes.CDLL:
         ("sonic_fused_multistep", MultistepArgs),
         ("sonic_bounded_topk", TopKArgs),
         ("sonic_fused_singular_static", SingularArgs),
+        ("sonic_cache_append", CacheAppendArgs),
+        ("sonic_cache_gather", CacheGatherArgs),
+        ("sonic_paged_attention", PagedAttentionArgs),
+        ("sonic_residual_norm", ResidualNormArgs),
     ):
         fn = getattr(lib, name)
         fn.argtypes = [ctypes.POINTER(argt), _vp]

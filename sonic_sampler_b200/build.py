@@ -12,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -19,17 +20,33 @@ CSRC = PACKAGE_DIR / "csrc"
 OUT = PACKAGE_DIR / "_lib" / "libsonic_b200.so"
 # diagnostic variant with per-phase timing stamps (python -m sonic_sampler_b200.phases)
 STAMPS_OUT = PACKAGE_DIR / "_lib" / "libsonic_b200_stamps.so"
-SOURCES = [CSRC / "sampler.cu"]
-HEADERS = [CSRC / "common.cuh", CSRC / "exports.map", PACKAGE_DIR.parent / "include" / "sonic_b200.h"]
+API = PACKAGE_DIR.parent / "include" / "sonic_b200.h"
+EXPORTS = CSRC / "exports.map"
+#: translation unit -> the headers it includes (each is compiled on its own, and again only when
+#: one of its files is newer than its object)
+UNITS = {
+    CSRC / "sampler.cu": [CSRC / "common.cuh", CSRC / "host.h", API],
+    CSRC / "cache.cu": [CSRC / "host.h", CSRC / "values.cuh", API],
+    CSRC / "attention.cu": [CSRC / "host.h", CSRC / "values.cuh", API],
+    CSRC / "norm.cu": [CSRC / "host.h", CSRC / "values.cuh", API],
+}
+SOURCES = list(UNITS)
+HEADERS = sorted({h for headers in UNITS.values() for h in headers} | {EXPORTS})
 
-NVCC_FLAGS = [
+COMPILE_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    # exact bf16/fp32 reproduction: no implicit multiply-add contraction
-    "--fmad=false",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "-cudart", "static",
-    "-Xlinker", f"--version-script={CSRC / 'exports.map'}",
+]
+#: flags of single units: the sampler reproduces bf16/fp32 results exactly, so no implicit
+#: multiply-add contraction there
+UNIT_FLAGS = {CSRC / "sampler.cu": ["--fmad=false"]}
+LINK_FLAGS = [
+    "-gencode", "arch=compute_100a,code=sm_100a",
+    "-shared", "-Xcompiler", "-fPIC",
+    "-cudart", "static",
+    "-Xlinker", f"--version-script={EXPORTS}",
 ]
 
 
@@ -56,13 +73,28 @@ def build(force: bool = False, verbose: bool = False, stamps: bool = False) -> P
     if not force and not stale(out):
         return out
     out.parent.mkdir(parents=True, exist_ok=True)
-    tmp = out.with_suffix(".so.tmp")
-    cmd = [nvcc_path(), *NVCC_FLAGS, *(["-DSONIC_PHASE_STAMPS"] if stamps else []), "-o", str(tmp),
-           *map(str, SOURCES)]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
-    os.replace(tmp, out)
+    define = ["-DSONIC_PHASE_STAMPS"] if stamps else []
+    objects, commands = [], []
+    for source, headers in UNITS.items():
+        # objects sit beside the library; only the sampler has a phase-stamp variant
+        suffix = "_stamps.o" if stamps and source.name == "sampler.cu" else ".o"
+        obj = out.parent / (source.stem + suffix)
+        objects.append(obj)
+        newest = max(p.stat().st_mtime for p in (source, *headers, Path(__file__)))
+        if force or not obj.is_file() or obj.stat().st_mtime < newest:
+            commands.append(([nvcc_path(), *COMPILE_FLAGS, *UNIT_FLAGS.get(source, []), *define, "-c", str(source)], obj))
+
+    def run(cmd, target):
+        tmp = target.with_suffix(target.suffix + ".tmp")
+        cmd = [*cmd, "-o", str(tmp)]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+        os.replace(tmp, target)
+
+    with ThreadPoolExecutor() as pool:
+        list(pool.map(lambda c: run(*c), commands))
+    run([nvcc_path(), *LINK_FLAGS, *map(str, objects)], out)
     return out
 
 

@@ -1,0 +1,272 @@
+// The paged key-value cache: new rows into their pages (quantised on the way), and pages read back
+// into rows. Both are copies bound by memory: a row is read once and written once.
+//
+// A CTA takes a run of consecutive token rows. Its first threads look the tokens up (request,
+// position, page), one token a thread, so the chain of dependent reads is paid once a CTA; then all
+// threads move 16-byte pieces, every (token, keys or values, head) row by a group of neighbouring
+// lanes.
+
+#include <algorithm>
+
+#include "host.h"
+#include "values.cuh"
+
+namespace sonic {
+namespace {
+
+constexpr int NT = 256;
+constexpr int MAX_RUN = 64;  // tokens a CTA takes at most
+
+// Request of row `row`: the last b with bounds[b] <= row (bounds non-decreasing, bounds[0] <= row).
+__device__ __forceinline__ int request_of(const int32_t* bounds, int requests, int row) {
+  int lo = 0, hi = requests - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (bounds[mid] <= row)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+// Element offset of (page, slot) in the pages, and of its scales; head 0.
+struct Slot {
+  int64_t at = -1;  // -1: nothing there
+  int64_t scale = 0;
+};
+
+__device__ __forceinline__ Slot find_slot(const SonicPagedCache& c, const SonicSequences& s, int request, int64_t position,
+                                          uint32_t* error) {
+  Slot found;
+  if (position < 0) return found;
+  const int64_t index = position / c.page_size;
+  int page = -1;
+  if (index < s.table_width) page = s.page_table[request * s.table_stride + index];
+  if (page < 0 || page >= c.pages) {
+    if (error) atomicOr(error, (uint32_t)SONIC_DEVICE_ERR_PAGE);
+    return found;
+  }
+  const int slot = (int)(position - index * c.page_size);
+  found.at = page * c.page_stride + slot * c.slot_stride;
+  found.scale = page * c.scale_page_stride + slot;
+  return found;
+}
+
+// Each thread moves 8 activations: 16 bytes in; 16 bytes (16-bit cache) or 8 codes out. A row is
+// head_dim / 8 neighbouring lanes (8, 16 or 32), which reduce its largest magnitude by shuffles.
+template <typename T, bool Q8>
+__global__ void __launch_bounds__(NT) append_kernel(SonicCacheAppendArgs a, int run, int row_shift) {
+  __shared__ Slot slots[MAX_RUN];
+  grid_dependency_trigger();
+  grid_dependency_wait();
+  const SonicSequences& s = a.sequences;
+  const SonicPagedCache& c = a.cache;
+  const int first = blockIdx.x * run;
+  const int count = min(run, s.tokens - first);
+  if (threadIdx.x < count) {
+    const int row = first + threadIdx.x;
+    Slot found;
+    if (s.cu_seqlens) {
+      const int b = request_of(s.cu_seqlens, s.requests, row);
+      // rows outside every request have no place in the cache
+      if (row >= s.cu_seqlens[b] && row < s.cu_seqlens[b + 1])
+        found = find_slot(c, s, b, (int64_t)s.lengths[b] - s.cu_seqlens[b + 1] + row, a.error);
+    } else {
+      const int each = s.tokens / s.requests, b = row / each;
+      found = find_slot(c, s, b, (int64_t)s.lengths[b] - each + row % each, a.error);
+    }
+    slots[threadIdx.x] = found;
+  }
+  __syncthreads();
+  const int lanes = 1 << row_shift;                  // lanes a row
+  const int rows = count * c.kv_heads * 2;           // (token, head, keys / values)
+  const int lane = threadIdx.x & (lanes - 1);
+  // all lanes of a warp make the same number of rounds: the shuffles below are warp-wide
+  const int rounds = (rows * lanes + NT - 1) / NT;
+  for (int i = 0; i < rounds; ++i) {
+    const int r = (i * NT + threadIdx.x) >> row_shift;
+    const bool live = r < rows;
+    const int half = r & 1, head = (r >> 1) % c.kv_heads, t = (r >> 1) / c.kv_heads;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    Slot slot;
+    if (live) {
+      slot = slots[t];
+      const int64_t at = half ? (first + t) * a.value_token_stride + head * a.value_head_stride
+                              : (first + t) * a.key_token_stride + head * a.key_head_stride;
+      x = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(half ? a.values : a.keys) + at + lane * 8));
+    }
+    void* pages = half ? c.values : c.keys;
+    const int64_t to = slot.at + head * c.head_stride + lane * 8;
+    if constexpr (!Q8) {
+      if (slot.at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(pages) + to) = x;
+    } else {
+      const float2 f0 = Pair<T>::unpack(x.x), f1 = Pair<T>::unpack(x.y), f2 = Pair<T>::unpack(x.z), f3 = Pair<T>::unpack(x.w);
+      uint32_t top = max(max(max(magnitude_bits(f0.x), magnitude_bits(f0.y)), max(magnitude_bits(f1.x), magnitude_bits(f1.y))),
+                         max(max(magnitude_bits(f2.x), magnitude_bits(f2.y)), max(magnitude_bits(f3.x), magnitude_bits(f3.y))));
+      for (int d = lanes >> 1; d >= 1; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+      float scale, inverse;
+      e4m3_scale(top, scale, inverse);
+      if (slot.at >= 0) {
+        const uint2 codes = make_uint2(e4m3_pack4(f0.x * inverse, f0.y * inverse, f1.x * inverse, f1.y * inverse),
+                                       e4m3_pack4(f2.x * inverse, f2.y * inverse, f3.x * inverse, f3.y * inverse));
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pages) + to) = codes;
+        if (lane == 0) (half ? c.value_scales : c.key_scales)[slot.scale + head * c.scale_head_stride] = scale;
+      }
+    }
+  }
+}
+
+// Each thread moves 16 cached bytes: 8 values of a 16-bit cache, or 16 codes into 32 bytes.
+template <typename T, bool Q8>
+__global__ void __launch_bounds__(NT) gather_kernel(SonicCacheGatherArgs a, int run, int row_shift) {
+  __shared__ Slot slots[MAX_RUN];
+  grid_dependency_trigger();
+  grid_dependency_wait();
+  const SonicSequences& s = a.sequences;
+  const SonicPagedCache& c = a.cache;
+  const int first = blockIdx.x * run;
+  const int count = min(run, s.tokens - first);
+  if (threadIdx.x < count) {
+    const int row = first + threadIdx.x;
+    const int b = request_of(a.starts, s.requests, row);
+    Slot found;
+    if (row >= a.starts[b] && row < a.starts[b + 1]) found = find_slot(c, s, b, row - a.starts[b], a.error);
+    slots[threadIdx.x] = found;
+  }
+  __syncthreads();
+  constexpr int PER = Q8 ? 16 : 8;  // values a thread
+  const int lanes = 1 << row_shift;
+  const int lane = threadIdx.x & (lanes - 1);
+  const int rows = count * c.kv_heads * 2;
+  for (int r = threadIdx.x >> row_shift; r < rows; r += NT >> row_shift) {
+    // heads innermost: the rows of a token are neighbours in the output
+    const int head = r % c.kv_heads, half = (r / c.kv_heads) & 1, t = r / (2 * c.kv_heads);
+    const Slot slot = slots[t];
+    uint4 x = make_uint4(0, 0, 0, 0);
+    float scale = 0.0f;
+    if (slot.at >= 0) {
+      const int64_t at = slot.at + head * c.head_stride + lane * PER;
+      const void* pages = half ? c.values : c.keys;
+      if constexpr (Q8) {
+        x = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pages) + at));
+        scale = __ldg((half ? c.value_scales : c.key_scales) + slot.scale + head * c.scale_head_stride);
+      } else {
+        x = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(pages) + at));
+      }
+    }
+    T* out = static_cast<T*>(half ? a.values : a.keys) +
+             ((int64_t)(first + t) * c.kv_heads + head) * c.head_dim + lane * PER;
+    if constexpr (!Q8) {
+      *reinterpret_cast<uint4*>(out) = x;
+    } else {
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      uint32_t y[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 lo = Pair<__half>::unpack(e4m3_to_half2((uint16_t)w[i]));
+        const float2 hi = Pair<__half>::unpack(e4m3_to_half2((uint16_t)(w[i] >> 16)));
+        y[2 * i] = Pair<T>::pack(lo.x * scale, lo.y * scale);
+        y[2 * i + 1] = Pair<T>::pack(hi.x * scale, hi.y * scale);
+      }
+      reinterpret_cast<uint4*>(out)[0] = make_uint4(y[0], y[1], y[2], y[3]);
+      reinterpret_cast<uint4*>(out)[1] = make_uint4(y[4], y[5], y[6], y[7]);
+    }
+  }
+}
+
+int log2_of(int v) {
+  int l = 0;
+  while ((1 << l) < v) ++l;
+  return l;
+}
+
+// Tokens a CTA takes: enough that a thread moves several pieces, few enough that a small call
+// still covers the SMs.
+int run_of(int tokens, int pieces_per_token) {
+  const int full = std::max(1, 4 * NT / pieces_per_token);
+  const int spread = std::max(1, tokens / 296);
+  return std::min(MAX_RUN, std::min(full, spread));
+}
+
+bool is_16bit(int dtype) { return dtype == SONIC_DTYPE_BF16 || dtype == SONIC_DTYPE_F16; }
+
+}  // namespace
+
+sonic_status check_cache(const SonicPagedCache& c) noexcept {
+  if (!c.keys || !c.values) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "cache keys and values must not be NULL");
+  if (!is_16bit(c.dtype) && c.dtype != SONIC_DTYPE_E4M3)
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "cache dtype must be bf16, f16 or e4m3");
+  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256)
+    return fail_with(SONIC_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256");
+  if (c.pages < 1 || c.page_size < 1 || c.kv_heads < 1)
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "pages, page_size and kv_heads must be positive");
+  if (c.kv_heads > 1024) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "kv_heads must be at most 1024");
+  const int per = c.dtype == SONIC_DTYPE_E4M3 ? 16 : 8;
+  if (!is_aligned(c.keys, 16) || !is_aligned(c.values, 16) || c.page_stride % per || c.head_stride % per || c.slot_stride % per)
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "cache rows must start on 16-byte boundaries");
+  if (c.page_stride < 0 || c.head_stride < 0 || c.slot_stride < 0 || c.scale_page_stride < 0 || c.scale_head_stride < 0)
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "cache strides must not be negative");
+  if (c.dtype == SONIC_DTYPE_E4M3 && (!c.key_scales || !c.value_scales))
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "an e4m3 cache needs key_scales and value_scales");
+  return SONIC_OK;
+}
+
+sonic_status check_sequences(const SonicSequences& s, bool lengths) noexcept {
+  if (s.requests < 1 || s.tokens < 0) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "requests must be positive and tokens not negative");
+  if (!s.page_table || s.table_width < 1 || s.table_stride < 0)
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "page_table must have at least one column");
+  if (lengths && !s.lengths) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "lengths must not be NULL");
+  if (lengths && !s.cu_seqlens && s.tokens % s.requests)
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "without cu_seqlens, tokens must be a multiple of requests");
+  return SONIC_OK;
+}
+
+}  // namespace sonic
+
+using namespace sonic;
+
+extern "C" sonic_status sonic_cache_append(const SonicCacheAppendArgs* a, void* stream) {
+  if (!a) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "args must not be NULL");
+  if (sonic_status s = check_cache(a->cache)) return s;
+  if (sonic_status s = check_sequences(a->sequences, true)) return s;
+  if (a->sequences.tokens == 0) return SONIC_OK;
+  if (!is_16bit(a->dtype) || (a->cache.dtype != SONIC_DTYPE_E4M3 && a->cache.dtype != a->dtype))
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "keys and values must be bf16 or f16, and of the cache's dtype unless it is e4m3");
+  if (!a->keys || !a->values) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "keys and values must not be NULL");
+  if (!is_aligned(a->keys, 16) || !is_aligned(a->values, 16) || a->key_token_stride % 8 || a->key_head_stride % 8 ||
+      a->value_token_stride % 8 || a->value_head_stride % 8)
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "rows of keys and values must start on 16-byte boundaries");
+  const int lanes = a->cache.head_dim / 8;
+  const int run = run_of(a->sequences.tokens, 2 * a->cache.kv_heads * lanes);
+  const dim3 grid((a->sequences.tokens + run - 1) / run);
+  const bool pdl = a->flags & SONIC_FLAG_PDL;
+  const auto go = [&](auto kernel) {
+    return launch_status(launch_kernel(kernel, grid, dim3(NT), 0, (cudaStream_t)stream, pdl, *a, run, log2_of(lanes)));
+  };
+  const bool q8 = a->cache.dtype == SONIC_DTYPE_E4M3;
+  if (a->dtype == SONIC_DTYPE_BF16) return q8 ? go(append_kernel<__nv_bfloat16, true>) : go(append_kernel<__nv_bfloat16, false>);
+  return q8 ? go(append_kernel<__half, true>) : go(append_kernel<__half, false>);
+}
+
+extern "C" sonic_status sonic_cache_gather(const SonicCacheGatherArgs* a, void* stream) {
+  if (!a) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "args must not be NULL");
+  if (sonic_status s = check_cache(a->cache)) return s;
+  if (sonic_status s = check_sequences(a->sequences, false)) return s;
+  if (a->sequences.tokens == 0) return SONIC_OK;
+  if (!is_16bit(a->dtype) || (a->cache.dtype != SONIC_DTYPE_E4M3 && a->cache.dtype != a->dtype))
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "outputs must be bf16 or f16, and of the cache's dtype unless it is e4m3");
+  if (!a->starts || !a->keys || !a->values) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "starts, keys and values must not be NULL");
+  if (!is_aligned(a->keys, 16) || !is_aligned(a->values, 16))
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "outputs must start on 16-byte boundaries");
+  const bool q8 = a->cache.dtype == SONIC_DTYPE_E4M3;
+  const int lanes = a->cache.head_dim / (q8 ? 16 : 8);
+  const int run = run_of(a->sequences.tokens, 2 * a->cache.kv_heads * lanes);
+  const dim3 grid((a->sequences.tokens + run - 1) / run);
+  const bool pdl = a->flags & SONIC_FLAG_PDL;
+  const auto go = [&](auto kernel) {
+    return launch_status(launch_kernel(kernel, grid, dim3(NT), 0, (cudaStream_t)stream, pdl, *a, run, log2_of(lanes)));
+  };
+  if (a->dtype == SONIC_DTYPE_BF16) return q8 ? go(gather_kernel<__nv_bfloat16, true>) : go(gather_kernel<__nv_bfloat16, false>);
+  return q8 ? go(gather_kernel<__half, true>) : go(gather_kernel<__half, false>);
+}

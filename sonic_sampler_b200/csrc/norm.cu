@@ -1,0 +1,293 @@
+// Residual root-mean-square norm: r = x + residual, y = r / sqrt(mean(r^2) + eps) * weight, with y
+// rounded to the input type or quantised to e4m3 with a scale per row or per 128 columns.
+//
+// Bound by memory: one pass, the row stays in registers between the sum of squares and the output.
+// A row belongs to one CTA, or to one warp where a warp's registers hold it, so that short rows pay
+// no block barrier. Each lane holds N items of P values: P consecutive ones in a 16-byte piece
+// where rows are aligned, else 4 values 32 columns apart (a warp then still reads consecutive
+// addresses, and an item of a warp is 128 consecutive columns in both layouts of a group).
+
+#include <algorithm>
+
+#include "host.h"
+#include "values.cuh"
+
+namespace sonic {
+namespace {
+
+constexpr int MAX_WARPS = 32;
+
+template <typename T>
+__device__ __forceinline__ float to_float(T x) {
+  if constexpr (sizeof(T) == 4)
+    return x;
+  else if constexpr (std::is_same<T, __half>::value)
+    return __half2float(x);
+  else
+    return __bfloat162float(x);
+}
+
+template <typename T>
+__device__ __forceinline__ T from_float(float x) {
+  if constexpr (sizeof(T) == 4)
+    return x;
+  else if constexpr (std::is_same<T, __half>::value)
+    return __float2half_rn(x);
+  else
+    return __float2bfloat16_rn(x);
+}
+
+// values of one 16-byte piece of a row
+template <typename T>
+struct Piece {
+  static constexpr int P = 16 / sizeof(T);
+  static __device__ __forceinline__ void unpack(const uint4& x, float (&f)[P]) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 v = Pair<T>::unpack(w[i]);
+        f[2 * i] = v.x;
+        f[2 * i + 1] = v.y;
+      }
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&f)[P]) {
+    if constexpr (sizeof(T) == 4)
+      return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    else
+      return make_uint4(Pair<T>::pack(f[0], f[1]), Pair<T>::pack(f[2], f[3]), Pair<T>::pack(f[4], f[5]), Pair<T>::pack(f[6], f[7]));
+  }
+};
+
+// Row statistics over the warps of a row (`warps` of them; 1: no block barrier).
+__device__ __forceinline__ float row_sum(float v, int warps, float* shared) {
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  if (warps == 1) return v;
+  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = (threadIdx.x & 31) < warps ? shared[threadIdx.x & 31] : 0.0f;
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+__device__ __forceinline__ uint32_t row_max(uint32_t v, int warps, uint32_t* shared) {
+  v = __reduce_max_sync(0xffffffffu, v);
+  if (warps == 1) return v;
+  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < warps ? shared[threadIdx.x & 31] : 0u);
+}
+
+// N: items a lane; VEC: 16-byte pieces. blockDim.x = 32 * warps of a row, blockDim.y = rows a CTA
+// (more than one only with one warp a row).
+template <typename T, bool Q8, bool VEC, int N>
+__global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
+  constexpr int P = VEC ? Piece<T>::P : 4;
+  __shared__ float sums[MAX_WARPS];
+  __shared__ uint32_t tops[MAX_WARPS];
+  grid_dependency_trigger();
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= a.rows) return;  // whole warps: a CTA with several rows has one warp a row
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
+  const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
+  const T* weight = static_cast<const T*>(a.weight);
+  T* res_out = a.residual_out ? static_cast<T*>(a.residual_out) + row * a.residual_out_stride : nullptr;
+
+  // column of value j of item i
+  const auto column = [&](int i, int j) {
+    if constexpr (VEC) return ((i * warps + warp) * 32 + lane) * P + j;
+    return (i * warps + warp) * 128 + lane + 32 * j;
+  };
+
+  float r[N][P];
+  grid_dependency_wait();
+  if constexpr (VEC) {
+    uint4 xs[N], rs[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      xs[i] = rs[i] = make_uint4(0, 0, 0, 0);
+      if (column(i, 0) < a.hidden) {
+        xs[i] = *reinterpret_cast<const uint4*>(x + column(i, 0));
+        if (res) rs[i] = *reinterpret_cast<const uint4*>(res + column(i, 0));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      Piece<T>::unpack(xs[i], r[i]);
+      if (res) {
+        float f[P];
+        Piece<T>::unpack(rs[i], f);
+#pragma unroll
+        for (int j = 0; j < P; ++j) r[i][j] += f[j];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const int at = column(i, j);
+        r[i][j] = at < a.hidden ? to_float(x[at]) + (res ? to_float(res[at]) : 0.0f) : 0.0f;
+      }
+  }
+  float sum = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < P; ++j) s = fmaf(r[i][j], r[i][j], s);
+    sum += s;
+  }
+  if (res_out) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (VEC) {
+        if (column(i, 0) < a.hidden) *reinterpret_cast<uint4*>(res_out + column(i, 0)) = Piece<T>::pack(r[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+          if (column(i, j) < a.hidden) res_out[column(i, j)] = from_float<T>(r[i][j]);
+      }
+    }
+  }
+  const float rstd = __frsqrt_rn(__fdiv_rn(row_sum(sum, warps, sums), (float)a.hidden) + a.eps);
+
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (VEC) {
+      float w[P];
+      uint4 ws = make_uint4(0, 0, 0, 0);
+      if (column(i, 0) < a.hidden) ws = __ldg(reinterpret_cast<const uint4*>(weight + column(i, 0)));
+      Piece<T>::unpack(ws, w);
+#pragma unroll
+      for (int j = 0; j < P; ++j) r[i][j] = column(i, 0) < a.hidden ? r[i][j] * rstd * w[j] : 0.0f;
+    } else {
+#pragma unroll
+      for (int j = 0; j < P; ++j)
+        r[i][j] = column(i, j) < a.hidden ? r[i][j] * rstd * to_float(weight[column(i, j)]) : 0.0f;
+    }
+  }
+
+  if constexpr (!Q8) {
+    T* out = static_cast<T*>(a.out) + row * a.out_stride;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if constexpr (VEC) {
+        if (column(i, 0) < a.hidden) *reinterpret_cast<uint4*>(out + column(i, 0)) = Piece<T>::pack(r[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+          if (column(i, j) < a.hidden) out[column(i, j)] = from_float<T>(r[i][j]);
+      }
+    }
+  } else {
+    uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.out_stride;
+    float scale, inverse;
+    if (a.group == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < P; ++j) top = max(top, magnitude_bits(r[i][j]));
+      e4m3_scale(row_max(top, warps, tops), scale, inverse);
+      if (threadIdx.x == 0) a.scales[row] = scale;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (a.group) {
+        // the item's 128 columns: 128 / P neighbouring lanes (the whole warp in the strided layout)
+        constexpr int LANES = VEC ? 128 / P : 32;
+        uint32_t t = 0;
+#pragma unroll
+        for (int j = 0; j < P; ++j) t = max(t, magnitude_bits(r[i][j]));
+#pragma unroll
+        for (int d = LANES / 2; d >= 1; d >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, d));
+        e4m3_scale(t, scale, inverse);
+        const int at = VEC ? column(i, 0) : (i * warps + warp) * 128;
+        if (at < a.hidden && lane % LANES == 0) a.scales[row * ((a.hidden + 127) / 128) + at / 128] = scale;
+      }
+      if constexpr (VEC) {
+        if (column(i, 0) < a.hidden) {
+          const uint32_t lo = e4m3_pack4(r[i][0] * inverse, r[i][1] * inverse, r[i][2] * inverse, r[i][3] * inverse);
+          if constexpr (P == 8) {
+            const uint32_t hi = e4m3_pack4(r[i][4] * inverse, r[i][5] * inverse, r[i][6] * inverse, r[i][7] * inverse);
+            *reinterpret_cast<uint2*>(out + column(i, 0)) = make_uint2(lo, hi);
+          } else {
+            *reinterpret_cast<uint32_t*>(out + column(i, 0)) = lo;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+          if (column(i, j) < a.hidden) out[column(i, j)] = (uint8_t)e4m3_pack2(r[i][j] * inverse, 0.0f);
+      }
+    }
+  }
+}
+
+template <typename T, bool Q8, bool VEC>
+sonic_status run(const SonicResidualNormArgs& a, cudaStream_t stream) {
+  constexpr int PER_WARP = 32 * (VEC ? Piece<T>::P : 4);
+  const int items = (a.hidden + PER_WARP - 1) / PER_WARP;  // items of a row, over its warps
+  // few rows: as many warps as items (latency); many rows: up to 4 items a lane, so that each
+  // thread has several loads in flight
+  int n = (int64_t)a.rows < 296 ? 1 : std::min(4, items);
+  n = n == 3 ? 4 : n;
+  while ((items + n - 1) / n > MAX_WARPS) n *= 2;
+  const int warps = (items + n - 1) / n;
+  const int rows = warps == 1 ? std::min(a.rows, 4) : 1;
+  const dim3 block(32 * warps, rows), grid((a.rows + rows - 1) / rows);
+  const bool pdl = a.flags & SONIC_FLAG_PDL;
+  const auto go = [&](auto kernel) { return launch_status(launch_kernel(kernel, grid, block, 0, stream, pdl, a)); };
+  switch (n) {
+    case 1: return go(norm_kernel<T, Q8, VEC, 1>);
+    case 2: return go(norm_kernel<T, Q8, VEC, 2>);
+    case 4: return go(norm_kernel<T, Q8, VEC, 4>);
+    default: return go(norm_kernel<T, Q8, VEC, 8>);
+  }
+}
+
+template <typename T>
+sonic_status run_type(const SonicResidualNormArgs& a, cudaStream_t stream) {
+  constexpr int P = Piece<T>::P;
+  const bool q8 = a.out_dtype == SONIC_DTYPE_E4M3;
+  bool vec = a.hidden % P == 0 && is_aligned(a.x, 16) && a.x_stride % P == 0 && is_aligned(a.weight, 16);
+  if (a.residual) vec = vec && is_aligned(a.residual, 16) && a.residual_stride % P == 0;
+  if (a.residual_out) vec = vec && is_aligned(a.residual_out, 16) && a.residual_out_stride % P == 0;
+  vec = vec && is_aligned(a.out, q8 ? P : 16) && a.out_stride % P == 0;
+  if (q8) return vec ? run<T, true, true>(a, stream) : run<T, true, false>(a, stream);
+  return vec ? run<T, false, true>(a, stream) : run<T, false, false>(a, stream);
+}
+
+}  // namespace
+}  // namespace sonic
+
+using namespace sonic;
+
+extern "C" sonic_status sonic_residual_norm(const SonicResidualNormArgs* a, void* stream) {
+  if (!a) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "args must not be NULL");
+  if (a->rows < 0) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "rows must not be negative");
+  if (a->hidden < 1) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "hidden must be positive");
+  if (a->hidden > 32768) return fail_with(SONIC_ERR_UNSUPPORTED, "hidden must be at most 32768");
+  if (a->dtype != SONIC_DTYPE_BF16 && a->dtype != SONIC_DTYPE_F16 && a->dtype != SONIC_DTYPE_F32)
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "dtype must be bf16, f16 or f32");
+  if (a->out_dtype != a->dtype && a->out_dtype != SONIC_DTYPE_E4M3)
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "out_dtype must be dtype or e4m3");
+  if (a->out_dtype == SONIC_DTYPE_E4M3 ? (a->group != 0 && a->group != 128) : a->group != 0)
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "group must be 0, or 128 with an e4m3 output");
+  if (a->rows == 0) return SONIC_OK;
+  if (!a->x || !a->weight || !a->out) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "x, weight and out must not be NULL");
+  if (a->out_dtype == SONIC_DTYPE_E4M3 && !a->scales)
+    return fail_with(SONIC_ERR_INVALID_ARGUMENT, "an e4m3 output needs scales");
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (a->dtype == SONIC_DTYPE_BF16) return run_type<__nv_bfloat16>(*a, st);
+  if (a->dtype == SONIC_DTYPE_F16) return run_type<__half>(*a, st);
+  return run_type<float>(*a, st);
+}

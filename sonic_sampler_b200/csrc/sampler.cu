@@ -32,6 +32,7 @@
 
 #include "../../include/sonic_b200.h"
 #include "common.cuh"
+#include "host.h"
 
 namespace sonic {
 
@@ -2825,6 +2826,14 @@ static thread_local std::string g_last_error;
 static sonic_status fail(sonic_status code, const std::string& msg) {
   g_last_error = msg;
   return code;
+}
+
+sonic_status fail_with(sonic_status code, const char* message) noexcept {
+  try {
+    return fail(code, message);
+  } catch (...) {
+    return code;  // no memory for the message
+  }
 }
 
 static bool aligned(const void* p, size_t a) { return ((uintptr_t)p % a) == 0; }

@@ -1,0 +1,81 @@
+"""`PagedAttention`: attention of a step's new tokens over a paged key-value cache.
+
+No counterpart in the reference, whose scope begins at the logits. One token a request is a decode
+step; `lookahead + 1` tokens a request, each seeing the keys up to its own, are the target model's
+side of a speculative verification (`UnshardedFusedMultistep` then judges its logits).
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import torch
+from torch import Tensor
+
+from sonic_sampler_b200 import ops
+from sonic_sampler_b200._abi import FLAG_PDL
+from sonic_sampler_b200.core.cache import PagedCache
+from sonic_sampler_b200.interface.base import default_device
+
+
+@dataclass(eq=False)
+class PagedAttention:
+    q_heads: int
+    kv_heads: int
+    head_dim: int
+    lookahead: int
+    pdl: bool
+    # zero-filled workspace of the kernel; calls that overlap on the GPU need objects of their own
+    scratchpad: Tensor
+
+    @classmethod
+    def initialize(cls, q_heads: int, kv_heads: int, head_dim: int, lookahead: int = 0, pdl: bool = True) -> "PagedAttention":
+        if q_heads < 1 or kv_heads < 1 or q_heads % kv_heads:
+            raise ValueError(f"q_heads must be a multiple of kv_heads, got {q_heads} and {kv_heads}")
+        if head_dim not in (64, 128, 256):
+            raise ValueError(f"head_dim must be 64, 128 or 256, got {head_dim}")
+        if lookahead < 0:
+            raise ValueError(f"lookahead must not be negative, got {lookahead}")
+        return cls(q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, lookahead=lookahead, pdl=pdl,
+                   scratchpad=ops.new_workspace(ops.paged_attention_workspace_bytes(), default_device()))
+
+    def device_error(self) -> int:
+        """Read and clear the device error word: 0, or DEVICE_ERR_PAGE when a call met a page id
+        outside the cache or a length outside its page-table row (that request's output is then
+        unspecified). Synchronises the current stream."""
+        return ops.workspace_error(self.scratchpad)
+
+    def __call__(self, queries: Tensor, cache: PagedCache, page_table: Tensor, lengths: Tensor,
+                 cu_seqlens: Tensor | None = None, window: int | None = None, scale: float | None = None,
+                 logsumexp: bool = False, output: Tensor | None = None) -> Tensor | tuple[Tensor, Tensor]:
+        """Attention of `queries` `[tokens, q_heads, head_dim]` (bf16 or fp16; the cache's dtype
+        unless it is e4m3) over the cached tokens of their requests, their own included.
+
+        Rows `cu_seqlens[b]:cu_seqlens[b + 1]` (without it, tokens / requests rows each) are the
+        last tokens of request b, which has `lengths[b]` in the cache. Each sees the keys up to its
+        own position, the last `window` of them where that is given. `scale` is 1 / sqrt(head_dim)
+        by default. `lookahead` of `initialize` is a hint: requests may bring more tokens.
+
+        Returns the output (in `output` where that is given), and with `logsumexp` also the fp32
+        `[tokens, q_heads]` logarithms of the softmax sums, with which outputs over disjoint key
+        ranges can be joined. A query that sees no key gives zeros and -infinity."""
+        ops._require_cuda(queries)
+        if queries.dim() != 3 or queries.size(1) != self.q_heads or queries.size(2) != self.head_dim:
+            raise ValueError(f"`queries` must be [tokens, {self.q_heads}, {self.head_dim}], got {list(queries.shape)}")
+        if cache.struct.kv_heads != self.kv_heads or cache.struct.head_dim != self.head_dim:
+            raise ValueError("the cache's kv_heads and head_dim must match `initialize`'s")
+        if window is not None and window < 1:
+            raise ValueError(f"`window` must be positive, got {window}")
+        device = cache.device
+        if self.scratchpad.device != device:
+            raise ValueError(f"the cache is on {device}, this object's workspace on {self.scratchpad.device}")
+        out = torch.empty(queries.shape, dtype=queries.dtype, device=device) if output is None else output
+        lse = torch.empty(queries.shape[:2], dtype=torch.float32, device=device) if logsumexp else None
+        args = ops.paged_attention_args(
+            cache.struct, queries, page_table, lengths, out, cu_seqlens=cu_seqlens,
+            max_tokens=self.lookahead + 1 if cu_seqlens is not None else 0, window=window or 0,
+            scale=1.0 / math.sqrt(self.head_dim) if scale is None else scale, lse=lse, flags=FLAG_PDL if self.pdl else 0,
+            workspace=self.scratchpad, device=device)
+        ops.launch_paged_attention(args, device)
+        return (out, lse) if logsumexp else out

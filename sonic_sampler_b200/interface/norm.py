@@ -1,0 +1,67 @@
+"""`ResidualNorm`: root-mean-square norm with the residual's addition and an output in 8 bits.
+
+No counterpart in the reference: it is the step between a served model's layers, and before the
+projection whose logits the sampler reads.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+from torch import Tensor
+
+from sonic_sampler_b200 import ops
+from sonic_sampler_b200._abi import FLAG_PDL
+
+E4M3 = torch.float8_e4m3fn
+
+
+@dataclass(eq=False)
+class ResidualNorm:
+    """r = x + residual, y = r / sqrt(mean(r^2) + eps) * weight, in fp32.
+
+    `dtype=torch.float8_e4m3fn` returns y's e4m3 codes, with an fp32 scale per row or per `group`
+    (128) columns: y stands for code * scale. Otherwise y is rounded to the input's dtype."""
+
+    weight: Tensor
+    eps: float = 1e-6
+    dtype: torch.dtype | None = None
+    group: int | None = None
+    pdl: bool = True
+
+    def __post_init__(self):
+        if self.dtype not in (None, E4M3, self.weight.dtype):
+            raise ValueError(f"`dtype` must be float8_e4m3fn or the weight's {self.weight.dtype}, got {self.dtype}")
+        if self.group not in (None, 128) or (self.group and self.dtype != E4M3):
+            raise ValueError(f"`group` must be 128 (with a float8_e4m3fn output) or None, got {self.group}")
+        if not self.eps >= 0.0:
+            raise ValueError(f"`eps` must not be negative, got {self.eps}")
+
+    def __call__(self, x: Tensor, residual: Tensor | None = None, residual_out: Tensor | None = None, out: Tensor | None = None,
+                 scales: Tensor | None = None) -> tuple[Tensor, Tensor | None, Tensor | None]:
+        """(y, scales, r) of rows `x` `[..., hidden]`, in the weight's dtype (bf16, fp16 or fp32).
+
+        `scales` is None unless the output is in 8 bits (`[..., 1]` or `[..., ceil(hidden / 128)]`);
+        r, rounded to the input's dtype, is None without a `residual`. `out`, `scales` and
+        `residual_out` may give the tensors to write; `residual_out` may be `residual` or `x`."""
+        ops._require_cuda(x)
+        shape, hidden = x.shape, self.weight.size(0)
+        if x.dim() < 1 or x.size(-1) != hidden:
+            raise ValueError(f"`x` must have {hidden} columns, got {list(shape)}")
+
+        def rows(t):
+            return t if t is None or t.dim() == 2 else t.view(-1, t.size(-1))
+
+        flat = rows(x)
+        if out is None:
+            out = torch.empty(shape, dtype=self.dtype or x.dtype, device=x.device)
+        if scales is None and out.dtype == E4M3:
+            groups = -(-hidden // self.group) if self.group else 1
+            scales = torch.empty((*shape[:-1], groups), dtype=torch.float32, device=x.device)
+        if residual is not None and residual_out is None:
+            residual_out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        args = ops.residual_norm_args(flat, self.weight, rows(out), residual=rows(residual), residual_out=rows(residual_out),
+                                      scales=rows(scales), eps=self.eps, group=self.group or 0, flags=FLAG_PDL if self.pdl else 0)
+        ops.launch_residual_norm(args, x.device)
+        return out, scales, residual_out

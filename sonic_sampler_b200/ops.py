@@ -17,11 +17,19 @@ from torch import Tensor
 from sonic_sampler_b200 import _abi
 from sonic_sampler_b200._abi import (
     DT_BF16,
+    DT_E4M3,
+    DT_F16,
     DT_F32,
     DT_I32,
     DT_I64,
+    CacheAppendArgs,
+    CacheGatherArgs,
     MultistepArgs,
+    PagedAttentionArgs,
+    PagedCacheStruct,
+    ResidualNormArgs,
     SamplingParams,
+    SequencesStruct,
     SingularArgs,
     TopKArgs,
 )
@@ -30,9 +38,14 @@ BF16 = torch.bfloat16
 F32 = torch.float32
 I32 = torch.int32
 I64 = torch.int64
+F16 = torch.float16
+E4M3 = torch.float8_e4m3fn
 
 _INDEX_DTYPES = {I32: DT_I32, I64: DT_I64}
 _FLOAT_DTYPES = {BF16: DT_BF16, F32: DT_F32}
+_ACTIVATION_DTYPES = {BF16: DT_BF16, F16: DT_F16}
+_CACHE_DTYPES = {BF16: DT_BF16, F16: DT_F16, E4M3: DT_E4M3}
+_NORM_DTYPES = {BF16: DT_BF16, F16: DT_F16, F32: DT_F32}
 
 
 def _ptr(t: Tensor | None) -> int | None:
@@ -433,3 +446,189 @@ def indexed_copy(source: Tensor, target: Tensor, indices: Tensor, indicator: Ten
             ctypes.c_void_p(source.data_ptr()), ctypes.c_void_p(target.data_ptr()), rows, source.stride(0), cols,
             source.element_size(), ctypes.c_void_p(indices.data_ptr()), index_dtype(indices, "indices"),
             indices.numel(), ctypes.c_void_p(indicator.data_ptr()), ctypes.c_void_p(_stream(source.device))), lib)
+
+
+# ---------------------------------------------------------------------------------------
+# decode-side operators: paged cache, attention over it, residual norm
+# ---------------------------------------------------------------------------------------
+
+
+def paged_cache_struct(keys: Tensor, values: Tensor, key_scales: Tensor | None, value_scales: Tensor | None) -> PagedCacheStruct:
+    """Descriptor of cache pages [pages, kv_heads, page_size, head_dim] (any strides but the inner
+    one) and, for e4m3 pages, their fp32 scales [pages, kv_heads, page_size]."""
+    _require(keys.dim() == 4 and keys.shape == values.shape, "cache keys and values must both be [pages, kv_heads, page_size, head_dim]")
+    _require(keys.dtype in _CACHE_DTYPES and values.dtype == keys.dtype, "cache keys and values must be bf16, fp16 or float8_e4m3fn")
+    _require(keys.device == values.device, "cache keys and values must be on one device")
+    _require(keys.stride() == values.stride() and keys.stride(3) == 1, "cache keys and values must share strides, with a unit inner one")
+    c = PagedCacheStruct()
+    c.pages, c.kv_heads, c.page_size, c.head_dim = keys.shape
+    c.page_stride, c.head_stride, c.slot_stride, _ = keys.stride()
+    c.dtype = _CACHE_DTYPES[keys.dtype]
+    c.keys, c.values = keys.data_ptr(), values.data_ptr()
+    if keys.dtype == E4M3:
+        _require(key_scales is not None and value_scales is not None, "a float8_e4m3fn cache needs key_scales and value_scales")
+        for name, t in (("key_scales", key_scales), ("value_scales", value_scales)):
+            _require(t.dtype == F32 and t.shape == keys.shape[:3] and t.device == keys.device and t.stride() == key_scales.stride()
+                     and (t.size(2) == 1 or t.stride(2) == 1),
+                     f"`{name}` must be fp32 [pages, kv_heads, page_size] on the cache's device, with a unit inner stride")
+        c.key_scales, c.value_scales = key_scales.data_ptr(), value_scales.data_ptr()
+        c.scale_page_stride, c.scale_head_stride = key_scales.stride(0), key_scales.stride(1)
+    else:
+        _require(key_scales is None and value_scales is None, "only a float8_e4m3fn cache has scales")
+    _keep(c, keys, values, key_scales, value_scales)
+    return c
+
+
+def _index_vector(t: Tensor, name: str, size: int, device: torch.device) -> int:
+    _require(t.dtype == I32 and t.dim() == 1 and t.size(0) == size and (size <= 1 or t.stride(0) == 1),
+             f"`{name}` must be a contiguous int32 vector of {size} entries")
+    _require(t.device == device, f"`{name}` must be on {device}")
+    return t.data_ptr()
+
+
+def _sequences(s: SequencesStruct, tokens: int, page_table: Tensor, lengths: Tensor | None, cu_seqlens: Tensor | None,
+               device: torch.device) -> None:
+    _require(page_table.dtype == I32 and page_table.dim() == 2 and (page_table.size(1) <= 1 or page_table.stride(1) == 1),
+             "`page_table` must be int32 [requests, pages] with a unit inner stride")
+    _require(page_table.device == device, f"`page_table` must be on {device}")
+    s.requests, s.table_width = page_table.shape
+    s.tokens = tokens
+    s.page_table, s.table_stride = page_table.data_ptr(), page_table.stride(0)
+    if lengths is not None:
+        s.lengths = _index_vector(lengths, "lengths", s.requests, device)
+        if cu_seqlens is not None:
+            s.cu_seqlens = _index_vector(cu_seqlens, "cu_seqlens", s.requests + 1, device)
+        else:
+            _require(s.requests > 0 and tokens % s.requests == 0, "without `cu_seqlens`, every request has the same number of tokens")
+
+
+def _token_rows(t: Tensor, name: str, heads: int, head_dim: int, device: torch.device) -> None:
+    _require(t.dim() == 3 and t.size(1) == heads and t.size(2) == head_dim and t.stride(2) == 1,
+             f"`{name}` must be [tokens, {heads}, {head_dim}] with a unit inner stride")
+    _require(t.device == device, f"`{name}` must be on {device}")
+
+
+def cache_append_args(cache: PagedCacheStruct, keys: Tensor, values: Tensor, page_table: Tensor, lengths: Tensor, *,
+                      cu_seqlens: Tensor | None, flags: int, error: Tensor | None, device: torch.device) -> CacheAppendArgs:
+    a = CacheAppendArgs()
+    a.cache = cache
+    _token_rows(keys, "keys", cache.kv_heads, cache.head_dim, device)
+    _token_rows(values, "values", cache.kv_heads, cache.head_dim, device)
+    _require(keys.size(0) == values.size(0), "`keys` and `values` must have the same number of tokens")
+    _require(keys.dtype in _ACTIVATION_DTYPES and values.dtype == keys.dtype, "`keys` and `values` must both be bf16 or fp16")
+    _sequences(a.sequences, keys.size(0), page_table, lengths, cu_seqlens, device)
+    a.flags = flags
+    a.dtype = _ACTIVATION_DTYPES[keys.dtype]
+    a.keys, a.values = keys.data_ptr(), values.data_ptr()
+    a.key_token_stride, a.key_head_stride, _ = keys.stride()
+    a.value_token_stride, a.value_head_stride, _ = values.stride()
+    a.error = _ptr(error)
+    _keep(a, keys, values, page_table, lengths, cu_seqlens, error)
+    return a
+
+
+def cache_gather_args(cache: PagedCacheStruct, page_table: Tensor, starts: Tensor, keys: Tensor, values: Tensor, *,
+                      flags: int, error: Tensor | None, device: torch.device) -> CacheGatherArgs:
+    a = CacheGatherArgs()
+    a.cache = cache
+    for name, t in (("keys", keys), ("values", values)):
+        _token_rows(t, name, cache.kv_heads, cache.head_dim, device)
+        _require(t.is_contiguous(), f"`{name}` must be contiguous")
+    _require(keys.size(0) == values.size(0), "`keys` and `values` must have the same number of rows")
+    _require(keys.dtype in _ACTIVATION_DTYPES and values.dtype == keys.dtype, "`keys` and `values` must both be bf16 or fp16")
+    _sequences(a.sequences, keys.size(0), page_table, None, None, device)
+    a.flags = flags
+    a.dtype = _ACTIVATION_DTYPES[keys.dtype]
+    a.starts = _index_vector(starts, "starts", page_table.size(0) + 1, device)
+    a.keys, a.values = keys.data_ptr(), values.data_ptr()
+    a.error = _ptr(error)
+    _keep(a, page_table, starts, keys, values, error)
+    return a
+
+
+def paged_attention_args(cache: PagedCacheStruct, queries: Tensor, page_table: Tensor, lengths: Tensor, out: Tensor, *,
+                         cu_seqlens: Tensor | None, max_tokens: int, window: int, scale: float, lse: Tensor | None, flags: int,
+                         workspace: Tensor | None, device: torch.device) -> PagedAttentionArgs:
+    a = PagedAttentionArgs()
+    a.cache = cache
+    _require(queries.dim() == 3, "`queries` must be [tokens, q_heads, head_dim]")
+    tokens, heads, _ = queries.shape
+    _token_rows(queries, "queries", heads, cache.head_dim, device)
+    _token_rows(out, "output", heads, cache.head_dim, device)
+    _require(out.size(0) == tokens and out.dtype == queries.dtype, "`output` must match `queries` in shape and dtype")
+    _require(queries.dtype in _ACTIVATION_DTYPES, "`queries` must be bf16 or fp16")
+    _sequences(a.sequences, tokens, page_table, lengths, cu_seqlens, device)
+    a.flags = flags
+    a.dtype = _ACTIVATION_DTYPES[queries.dtype]
+    a.q_heads, a.max_tokens, a.window, a.scale = heads, max_tokens, window, scale
+    a.queries, a.out = queries.data_ptr(), out.data_ptr()
+    a.q_token_stride, a.q_head_stride, _ = queries.stride()
+    a.out_token_stride, a.out_head_stride, _ = out.stride()
+    if lse is not None:
+        _require(lse.dtype == F32 and lse.shape == (tokens, heads) and lse.is_contiguous() and lse.device == device,
+                 "`logsumexp` must be a contiguous fp32 [tokens, q_heads] tensor on the queries' device")
+        a.lse = lse.data_ptr()
+    if workspace is not None:
+        a.workspace = workspace.data_ptr()
+        a.workspace_bytes = workspace.numel() * workspace.element_size()
+    _keep(a, queries, page_table, lengths, cu_seqlens, out, lse, workspace)
+    return a
+
+
+def _norm_rows(t: Tensor, name: str, rows: int, hidden: int, dtype: torch.dtype, device: torch.device) -> tuple[int, int]:
+    _require(t.dim() == 2 and t.size(0) == rows and t.size(1) == hidden and (hidden == 1 or t.stride(1) == 1),
+             f"`{name}` must be [{rows}, {hidden}] with a unit inner stride")
+    _require(t.dtype == dtype and t.device == device, f"`{name}` must be {dtype} on {device}")
+    return t.data_ptr(), t.stride(0)
+
+
+def residual_norm_args(x: Tensor, weight: Tensor, out: Tensor, *, residual: Tensor | None, residual_out: Tensor | None,
+                       scales: Tensor | None, eps: float, group: int, flags: int) -> ResidualNormArgs:
+    a = ResidualNormArgs()
+    _require(x.dim() == 2 and x.dtype in _NORM_DTYPES, "`x` must be a bf16, fp16 or fp32 [rows, hidden] tensor")
+    rows, hidden = x.shape
+    a.rows, a.hidden, a.dtype, a.group, a.flags, a.eps = rows, hidden, _NORM_DTYPES[x.dtype], group, flags, eps
+    a.x, a.x_stride = _norm_rows(x, "x", rows, hidden, x.dtype, x.device)
+    _require(weight.dim() == 1 and weight.size(0) == hidden and weight.dtype == x.dtype and weight.device == x.device
+             and (hidden == 1 or weight.stride(0) == 1), f"`weight` must be a contiguous {x.dtype} vector of {hidden} entries on {x.device}")
+    a.weight = weight.data_ptr()
+    if residual is not None:
+        a.residual, a.residual_stride = _norm_rows(residual, "residual", rows, hidden, x.dtype, x.device)
+    if residual_out is not None:
+        a.residual_out, a.residual_out_stride = _norm_rows(residual_out, "residual_out", rows, hidden, x.dtype, x.device)
+    _require(out.dtype in (x.dtype, E4M3), "`out` must have the dtype of `x`, or be float8_e4m3fn")
+    a.out_dtype = DT_E4M3 if out.dtype == E4M3 else a.dtype
+    a.out, a.out_stride = _norm_rows(out, "out", rows, hidden, out.dtype, x.device)
+    if out.dtype == E4M3:
+        groups = -(-hidden // group) if group else 1
+        _require(scales is not None and scales.dtype == F32 and scales.shape == (rows, groups) and scales.is_contiguous()
+                 and scales.device == x.device, f"`scales` must be a contiguous fp32 [{rows}, {groups}] tensor on {x.device}")
+        a.scales = scales.data_ptr()
+    _keep(a, x, weight, out, residual, residual_out, scales)
+    return a
+
+
+def paged_attention_workspace_bytes() -> int:
+    return int(_abi.load_library().sonic_paged_attention_workspace_size(ctypes.byref(PagedAttentionArgs())))
+
+
+def _launch(name: str, args, device: torch.device) -> None:
+    lib = _abi.load_library()
+    with torch.cuda.device(device):
+        _abi.check(getattr(lib, name)(ctypes.byref(args), ctypes.c_void_p(_stream(device))), lib)
+
+
+def launch_cache_append(args: CacheAppendArgs, device: torch.device) -> None:
+    _launch("sonic_cache_append", args, device)
+
+
+def launch_cache_gather(args: CacheGatherArgs, device: torch.device) -> None:
+    _launch("sonic_cache_gather", args, device)
+
+
+def launch_paged_attention(args: PagedAttentionArgs, device: torch.device) -> None:
+    _launch("sonic_paged_attention", args, device)
+
+
+def launch_residual_norm(args: ResidualNormArgs, device: torch.device) -> None:
+    _launch("sonic_residual_norm", args, device)
