@@ -27,7 +27,9 @@ EXPORTS = CSRC / "exports.map"
 UNITS = {
     CSRC / "sampler.cu": [CSRC / "common.cuh", CSRC / "host.h", API],
     CSRC / "cache.cu": [CSRC / "host.h", CSRC / "values.cuh", API],
-    CSRC / "attention.cu": [CSRC / "host.h", CSRC / "values.cuh", API],
+    CSRC / "attention.cu": [CSRC / "attention.h", CSRC / "host.h", API],
+    **{CSRC / f"attention_{types}.cu": [CSRC / "attention_kernel.cuh", CSRC / "attention.h", CSRC / "host.h", CSRC / "values.cuh", API]
+       for types in ("bf16", "f16", "bf16_e4m3", "f16_e4m3")},
     CSRC / "norm.cu": [CSRC / "host.h", CSRC / "values.cuh", API],
 }
 SOURCES = list(UNITS)

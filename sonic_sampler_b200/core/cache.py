@@ -38,6 +38,7 @@ class PagedCache:
     def __post_init__(self):
         self.struct = ops.paged_cache_struct(self.keys, self.values, self.key_scales, self.value_scales)
         self.device = self.keys.device
+        self.flags = FLAG_PDL if self.pdl else 0
         # the device error word of append and gather
         self.errors = ops.new_workspace(256, self.device)
 
@@ -66,7 +67,7 @@ class PagedCache:
         (`device_error`)."""
         ops._require_cuda(keys)
         args = ops.cache_append_args(self.struct, keys, values, page_table, lengths, cu_seqlens=cu_seqlens,
-                                     flags=FLAG_PDL if self.pdl else 0, error=self.errors, device=self.device)
+                                     flags=self.flags, error=self.errors, device=self.device)
         ops.launch_cache_append(args, self.device)
         return self
 
@@ -81,10 +82,10 @@ class PagedCache:
         ops._require_cuda(page_table)
         if dtype is None:
             dtype = keys.dtype if keys is not None else torch.bfloat16 if self.keys.dtype == E4M3 else self.keys.dtype
-        shape = (total, self.keys.size(1), self.keys.size(3))
-        keys = torch.empty(shape, dtype=dtype, device=self.device) if keys is None else keys
-        values = torch.empty(shape, dtype=dtype, device=self.device) if values is None else values
-        args = ops.cache_gather_args(self.struct, page_table, starts, keys, values, flags=FLAG_PDL if self.pdl else 0,
+        shape = (total, self.struct.kv_heads, self.struct.head_dim)
+        keys = self.keys.new_empty(shape, dtype=dtype) if keys is None else keys
+        values = self.keys.new_empty(shape, dtype=dtype) if values is None else values
+        args = ops.cache_gather_args(self.struct, page_table, starts, keys, values, flags=self.flags,
                                      error=self.errors, device=self.device)
         ops.launch_cache_gather(args, self.device)
         return keys, values

@@ -1,0 +1,51 @@
+// What the units of the paged attention share: the workspace's layout, and a launch by types.
+#pragma once
+
+#include "host.h"
+
+namespace sonic {
+
+constexpr int WARPS = 4;                   // of a CTA
+constexpr int MAX_CTAS = 296;              // 148 SMs x 2
+constexpr int MAX_WARPS = MAX_CTAS * WARPS;
+constexpr int PART_FLOATS = 4096;          // a partial result: 8 NT query rows x head_dim at most
+constexpr int PART_ROWS = 32;
+
+// Partial results: slots [0, 2 MAX_WARPS) hold what a warp has of the first and the last unit of its
+// share, slots [2 MAX_WARPS, 2 MAX_WARPS + 2 MAX_CTAS) what a CTA has of its own.
+constexpr int SLOTS = 2 * MAX_WARPS + 2 * MAX_CTAS;
+struct AttentionWorkspace {
+  uint32_t* error;
+  uint32_t* tickets;  // [2][2 * MAX_CTAS], zero between calls
+  float2* stats;      // [SLOTS][PART_ROWS] (m, l)
+  float4* parts;      // [SLOTS][PART_FLOATS / 4], in the order of the accumulator fragments
+};
+
+constexpr size_t HEADER = 256;             // error word
+constexpr size_t TICKET_BYTES = (size_t)4 * MAX_CTAS * 4 + 128;
+constexpr size_t STAT_BYTES = (size_t)SLOTS * PART_ROWS * 8;
+constexpr size_t PART_BYTES = (size_t)SLOTS * PART_FLOATS * 4;
+constexpr size_t WORKSPACE_BYTES = HEADER + TICKET_BYTES + STAT_BYTES + PART_BYTES;
+static_assert((HEADER + TICKET_BYTES) % 128 == 0 && STAT_BYTES % 128 == 0, "partial results are 16-byte aligned");
+
+struct AttentionLaunch {
+  SonicPagedAttentionArgs a;
+  AttentionWorkspace ws;
+  int group;               // query heads a kv head
+  uint32_t group_inverse;  // floor(2^32 / group) + 1: r / group is the high half of r times it
+  int page_shift;          // log2(page_size), or -1
+  int packed;              // a page's rows follow one another, and a page holds a multiple of 16 (1) or 32 (2)
+  int room;                // longest request: what a page-table row holds, at most 2^30
+  int window;              // 0 where no request is longer than it
+  int each;                // new tokens a request has, without cu_seqlens
+  int most;                // new tokens a request has at most, as far as the host knows
+  int direct;              // 0: balanced shares; else one CTA for each of this many row tiles a unit
+};
+
+// The kernel for the types of a call (one translation unit each).
+sonic_status attention_bf16(const AttentionLaunch& p, cudaStream_t stream);
+sonic_status attention_f16(const AttentionLaunch& p, cudaStream_t stream);
+sonic_status attention_bf16_e4m3(const AttentionLaunch& p, cudaStream_t stream);
+sonic_status attention_f16_e4m3(const AttentionLaunch& p, cudaStream_t stream);
+
+}  // namespace sonic

@@ -1,0 +1,7 @@
+// Paged attention: bf16 queries over an e4m3 cache.
+
+#include "attention_kernel.cuh"
+
+sonic_status sonic::attention_bf16_e4m3(const AttentionLaunch& p, cudaStream_t stream) {
+  return launch_shape<__nv_bfloat16, true>(p, stream);
+}

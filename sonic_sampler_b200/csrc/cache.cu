@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(NT) append_kernel(SonicCacheAppendArgs a, int 
       slot = slots[t];
       const int64_t at = half ? (first + t) * a.value_token_stride + head * a.value_head_stride
                               : (first + t) * a.key_token_stride + head * a.key_head_stride;
-      x = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(half ? a.values : a.keys) + at + lane * 8));
+      x = *reinterpret_cast<const uint4*>(static_cast<const T*>(half ? a.values : a.keys) + at + lane * 8);
     }
     void* pages = half ? c.values : c.keys;
     const int64_t to = slot.at + head * c.head_stride + lane * 8;
@@ -149,10 +149,10 @@ __global__ void __launch_bounds__(NT) gather_kernel(SonicCacheGatherArgs a, int 
       const int64_t at = slot.at + head * c.head_stride + lane * PER;
       const void* pages = half ? c.values : c.keys;
       if constexpr (Q8) {
-        x = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pages) + at));
-        scale = __ldg((half ? c.value_scales : c.key_scales) + slot.scale + head * c.scale_head_stride);
+        x = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pages) + at);
+        scale = (half ? c.value_scales : c.key_scales)[slot.scale + head * c.scale_head_stride];
       } else {
-        x = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(pages) + at));
+        x = *reinterpret_cast<const uint4*>(static_cast<const T*>(pages) + at);
       }
     }
     T* out = static_cast<T*>(half ? a.values : a.keys) +

@@ -61,20 +61,22 @@ class PagedAttention:
         `[tokens, q_heads]` logarithms of the softmax sums, with which outputs over disjoint key
         ranges can be joined. A query that sees no key gives zeros and -infinity."""
         ops._require_cuda(queries)
-        if queries.dim() != 3 or queries.size(1) != self.q_heads or queries.size(2) != self.head_dim:
-            raise ValueError(f"`queries` must be [tokens, {self.q_heads}, {self.head_dim}], got {list(queries.shape)}")
-        if cache.struct.kv_heads != self.kv_heads or cache.struct.head_dim != self.head_dim:
+        shape, struct, device = queries.shape, cache.struct, cache.device
+        if len(shape) != 3 or shape[1] != self.q_heads or shape[2] != self.head_dim:
+            raise ValueError(f"`queries` must be [tokens, {self.q_heads}, {self.head_dim}], got {list(shape)}")
+        if struct.kv_heads != self.kv_heads or struct.head_dim != self.head_dim:
             raise ValueError("the cache's kv_heads and head_dim must match `initialize`'s")
-        if window is not None and window < 1:
+        if window is None:
+            window = 0
+        elif window < 1:
             raise ValueError(f"`window` must be positive, got {window}")
-        device = cache.device
         if self.scratchpad.device != device:
             raise ValueError(f"the cache is on {device}, this object's workspace on {self.scratchpad.device}")
-        out = torch.empty(queries.shape, dtype=queries.dtype, device=device) if output is None else output
-        lse = torch.empty(queries.shape[:2], dtype=torch.float32, device=device) if logsumexp else None
+        out = queries.new_empty(shape) if output is None else output
+        lse = queries.new_empty(shape[:2], dtype=torch.float32) if logsumexp else None
         args = ops.paged_attention_args(
-            cache.struct, queries, page_table, lengths, out, cu_seqlens=cu_seqlens,
-            max_tokens=self.lookahead + 1 if cu_seqlens is not None else 0, window=window or 0,
+            struct, queries, page_table, lengths, out, cu_seqlens=cu_seqlens,
+            max_tokens=self.lookahead + 1 if cu_seqlens is not None else 0, window=window,
             scale=1.0 / math.sqrt(self.head_dim) if scale is None else scale, lse=lse, flags=FLAG_PDL if self.pdl else 0,
             workspace=self.scratchpad, device=device)
         ops.launch_paged_attention(args, device)

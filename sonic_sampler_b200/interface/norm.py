@@ -46,22 +46,20 @@ class ResidualNorm:
         r, rounded to the input's dtype, is None without a `residual`. `out`, `scales` and
         `residual_out` may give the tensors to write; `residual_out` may be `residual` or `x`."""
         ops._require_cuda(x)
-        shape, hidden = x.shape, self.weight.size(0)
-        if x.dim() < 1 or x.size(-1) != hidden:
+        shape, hidden = x.shape, self.weight.shape[0]
+        if not shape or shape[-1] != hidden:
             raise ValueError(f"`x` must have {hidden} columns, got {list(shape)}")
-
-        def rows(t):
-            return t if t is None or t.dim() == 2 else t.view(-1, t.size(-1))
-
-        flat = rows(x)
         if out is None:
-            out = torch.empty(shape, dtype=self.dtype or x.dtype, device=x.device)
+            out = x.new_empty(shape, dtype=self.dtype)
         if scales is None and out.dtype == E4M3:
             groups = -(-hidden // self.group) if self.group else 1
-            scales = torch.empty((*shape[:-1], groups), dtype=torch.float32, device=x.device)
+            scales = x.new_empty((*shape[:-1], groups), dtype=torch.float32)
         if residual is not None and residual_out is None:
-            residual_out = torch.empty(shape, dtype=x.dtype, device=x.device)
-        args = ops.residual_norm_args(flat, self.weight, rows(out), residual=rows(residual), residual_out=rows(residual_out),
-                                      scales=rows(scales), eps=self.eps, group=self.group or 0, flags=FLAG_PDL if self.pdl else 0)
+            residual_out = x.new_empty(shape)
+        flat = (x, out, residual, residual_out, scales)
+        if len(shape) != 2:
+            flat = [t if t is None else t.view(-1, t.size(-1)) for t in flat]
+        args = ops.residual_norm_args(flat[0], self.weight, flat[1], residual=flat[2], residual_out=flat[3], scales=flat[4],
+                                      eps=self.eps, group=self.group or 0, flags=FLAG_PDL if self.pdl else 0)
         ops.launch_residual_norm(args, x.device)
         return out, scales, residual_out

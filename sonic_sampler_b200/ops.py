@@ -479,70 +479,96 @@ def paged_cache_struct(keys: Tensor, values: Tensor, key_scales: Tensor | None, 
     return c
 
 
+# The builders below run once a call of a decode step: messages are formatted only where a check
+# fails, and each attribute of a tensor is asked for once.
+
+
 def _index_vector(t: Tensor, name: str, size: int, device: torch.device) -> int:
-    _require(t.dtype == I32 and t.dim() == 1 and t.size(0) == size and (size <= 1 or t.stride(0) == 1),
-             f"`{name}` must be a contiguous int32 vector of {size} entries")
-    _require(t.device == device, f"`{name}` must be on {device}")
+    if t.dtype != I32 or t.shape != (size,) or (size > 1 and t.stride(0) != 1):
+        raise ValueError(f"`{name}` must be a contiguous int32 vector of {size} entries")
+    if t.device != device:
+        raise ValueError(f"`{name}` must be on {device}")
     return t.data_ptr()
 
 
 def _sequences(s: SequencesStruct, tokens: int, page_table: Tensor, lengths: Tensor | None, cu_seqlens: Tensor | None,
-               device: torch.device) -> None:
-    _require(page_table.dtype == I32 and page_table.dim() == 2 and (page_table.size(1) <= 1 or page_table.stride(1) == 1),
-             "`page_table` must be int32 [requests, pages] with a unit inner stride")
-    _require(page_table.device == device, f"`page_table` must be on {device}")
-    s.requests, s.table_width = page_table.shape
+               device: torch.device) -> int:
+    """Fill `s`; returns the number of requests."""
+    shape = page_table.shape
+    if page_table.dtype != I32 or len(shape) != 2:
+        raise ValueError("`page_table` must be int32 [requests, pages] with a unit inner stride")
+    requests, width = shape
+    row, inner = page_table.stride()
+    if inner != 1 and width > 1:
+        raise ValueError("`page_table` must be int32 [requests, pages] with a unit inner stride")
+    if page_table.device != device:
+        raise ValueError(f"`page_table` must be on {device}")
+    s.requests = requests
+    s.table_width = width
+    s.table_stride = row
     s.tokens = tokens
-    s.page_table, s.table_stride = page_table.data_ptr(), page_table.stride(0)
+    s.page_table = page_table.data_ptr()
     if lengths is not None:
-        s.lengths = _index_vector(lengths, "lengths", s.requests, device)
+        s.lengths = _index_vector(lengths, "lengths", requests, device)
         if cu_seqlens is not None:
-            s.cu_seqlens = _index_vector(cu_seqlens, "cu_seqlens", s.requests + 1, device)
-        else:
-            _require(s.requests > 0 and tokens % s.requests == 0, "without `cu_seqlens`, every request has the same number of tokens")
+            s.cu_seqlens = _index_vector(cu_seqlens, "cu_seqlens", requests + 1, device)
+        elif requests == 0 or tokens % requests:
+            raise ValueError("without `cu_seqlens`, every request has the same number of tokens")
+    return requests
 
 
-def _token_rows(t: Tensor, name: str, heads: int, head_dim: int, device: torch.device) -> None:
-    _require(t.dim() == 3 and t.size(1) == heads and t.size(2) == head_dim and t.stride(2) == 1,
-             f"`{name}` must be [tokens, {heads}, {head_dim}] with a unit inner stride")
-    _require(t.device == device, f"`{name}` must be on {device}")
+def _token_rows(t: Tensor, name: str, heads: int, head_dim: int, device: torch.device) -> tuple[int, int, int]:
+    """(tokens, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim or stride[2] != 1:
+        raise ValueError(f"`{name}` must be [tokens, {heads}, {head_dim}] with a unit inner stride")
+    if t.device != device:
+        raise ValueError(f"`{name}` must be on {device}")
+    return shape[0], stride[0], stride[1]
 
 
 def cache_append_args(cache: PagedCacheStruct, keys: Tensor, values: Tensor, page_table: Tensor, lengths: Tensor, *,
                       cu_seqlens: Tensor | None, flags: int, error: Tensor | None, device: torch.device) -> CacheAppendArgs:
     a = CacheAppendArgs()
+    heads, dim = cache.kv_heads, cache.head_dim
+    tokens, a.key_token_stride, a.key_head_stride = _token_rows(keys, "keys", heads, dim, device)
+    rows, a.value_token_stride, a.value_head_stride = _token_rows(values, "values", heads, dim, device)
+    if rows != tokens:
+        raise ValueError("`keys` and `values` must have the same number of tokens")
+    dtype = keys.dtype
+    if dtype not in _ACTIVATION_DTYPES or values.dtype != dtype:
+        raise ValueError("`keys` and `values` must both be bf16 or fp16")
+    _sequences(a.sequences, tokens, page_table, lengths, cu_seqlens, device)
     a.cache = cache
-    _token_rows(keys, "keys", cache.kv_heads, cache.head_dim, device)
-    _token_rows(values, "values", cache.kv_heads, cache.head_dim, device)
-    _require(keys.size(0) == values.size(0), "`keys` and `values` must have the same number of tokens")
-    _require(keys.dtype in _ACTIVATION_DTYPES and values.dtype == keys.dtype, "`keys` and `values` must both be bf16 or fp16")
-    _sequences(a.sequences, keys.size(0), page_table, lengths, cu_seqlens, device)
     a.flags = flags
-    a.dtype = _ACTIVATION_DTYPES[keys.dtype]
-    a.keys, a.values = keys.data_ptr(), values.data_ptr()
-    a.key_token_stride, a.key_head_stride, _ = keys.stride()
-    a.value_token_stride, a.value_head_stride, _ = values.stride()
+    a.dtype = _ACTIVATION_DTYPES[dtype]
+    a.keys = keys.data_ptr()
+    a.values = values.data_ptr()
     a.error = _ptr(error)
-    _keep(a, keys, values, page_table, lengths, cu_seqlens, error)
+    a._tensors = (cache, keys, values, page_table, lengths, cu_seqlens, error)
     return a
 
 
 def cache_gather_args(cache: PagedCacheStruct, page_table: Tensor, starts: Tensor, keys: Tensor, values: Tensor, *,
                       flags: int, error: Tensor | None, device: torch.device) -> CacheGatherArgs:
     a = CacheGatherArgs()
+    heads, dim = cache.kv_heads, cache.head_dim
+    tokens, _, _ = _token_rows(keys, "keys", heads, dim, device)
+    rows, _, _ = _token_rows(values, "values", heads, dim, device)
+    if rows != tokens:
+        raise ValueError("`keys` and `values` must have the same number of rows")
+    dtype = keys.dtype
+    if dtype not in _ACTIVATION_DTYPES or values.dtype != dtype or not keys.is_contiguous() or not values.is_contiguous():
+        raise ValueError("`keys` and `values` must both be contiguous and bf16 or fp16")
+    requests = _sequences(a.sequences, tokens, page_table, None, None, device)
+    a.starts = _index_vector(starts, "starts", requests + 1, device)
     a.cache = cache
-    for name, t in (("keys", keys), ("values", values)):
-        _token_rows(t, name, cache.kv_heads, cache.head_dim, device)
-        _require(t.is_contiguous(), f"`{name}` must be contiguous")
-    _require(keys.size(0) == values.size(0), "`keys` and `values` must have the same number of rows")
-    _require(keys.dtype in _ACTIVATION_DTYPES and values.dtype == keys.dtype, "`keys` and `values` must both be bf16 or fp16")
-    _sequences(a.sequences, keys.size(0), page_table, None, None, device)
     a.flags = flags
-    a.dtype = _ACTIVATION_DTYPES[keys.dtype]
-    a.starts = _index_vector(starts, "starts", page_table.size(0) + 1, device)
-    a.keys, a.values = keys.data_ptr(), values.data_ptr()
+    a.dtype = _ACTIVATION_DTYPES[dtype]
+    a.keys = keys.data_ptr()
+    a.values = values.data_ptr()
     a.error = _ptr(error)
-    _keep(a, page_table, starts, keys, values, error)
+    a._tensors = (cache, page_table, starts, keys, values, error)
     return a
 
 
@@ -550,61 +576,82 @@ def paged_attention_args(cache: PagedCacheStruct, queries: Tensor, page_table: T
                          cu_seqlens: Tensor | None, max_tokens: int, window: int, scale: float, lse: Tensor | None, flags: int,
                          workspace: Tensor | None, device: torch.device) -> PagedAttentionArgs:
     a = PagedAttentionArgs()
-    a.cache = cache
-    _require(queries.dim() == 3, "`queries` must be [tokens, q_heads, head_dim]")
-    tokens, heads, _ = queries.shape
-    _token_rows(queries, "queries", heads, cache.head_dim, device)
-    _token_rows(out, "output", heads, cache.head_dim, device)
-    _require(out.size(0) == tokens and out.dtype == queries.dtype, "`output` must match `queries` in shape and dtype")
-    _require(queries.dtype in _ACTIVATION_DTYPES, "`queries` must be bf16 or fp16")
+    dim = cache.head_dim
+    heads = queries.shape[1] if queries.dim() == 3 else -1
+    tokens, a.q_token_stride, a.q_head_stride = _token_rows(queries, "queries", heads, dim, device)
+    rows, a.out_token_stride, a.out_head_stride = _token_rows(out, "output", heads, dim, device)
+    dtype = queries.dtype
+    if rows != tokens or out.dtype != dtype:
+        raise ValueError("`output` must match `queries` in shape and dtype")
+    if dtype not in _ACTIVATION_DTYPES:
+        raise ValueError("`queries` must be bf16 or fp16")
     _sequences(a.sequences, tokens, page_table, lengths, cu_seqlens, device)
+    a.cache = cache
     a.flags = flags
-    a.dtype = _ACTIVATION_DTYPES[queries.dtype]
-    a.q_heads, a.max_tokens, a.window, a.scale = heads, max_tokens, window, scale
-    a.queries, a.out = queries.data_ptr(), out.data_ptr()
-    a.q_token_stride, a.q_head_stride, _ = queries.stride()
-    a.out_token_stride, a.out_head_stride, _ = out.stride()
+    a.dtype = _ACTIVATION_DTYPES[dtype]
+    a.q_heads = heads
+    a.max_tokens = max_tokens
+    a.window = window
+    a.scale = scale
+    a.queries = queries.data_ptr()
+    a.out = out.data_ptr()
     if lse is not None:
-        _require(lse.dtype == F32 and lse.shape == (tokens, heads) and lse.is_contiguous() and lse.device == device,
-                 "`logsumexp` must be a contiguous fp32 [tokens, q_heads] tensor on the queries' device")
+        if lse.dtype != F32 or lse.shape != (tokens, heads) or not lse.is_contiguous() or lse.device != device:
+            raise ValueError("`logsumexp` must be a contiguous fp32 [tokens, q_heads] tensor on the queries' device")
         a.lse = lse.data_ptr()
     if workspace is not None:
         a.workspace = workspace.data_ptr()
-        a.workspace_bytes = workspace.numel() * workspace.element_size()
-    _keep(a, queries, page_table, lengths, cu_seqlens, out, lse, workspace)
+        a.workspace_bytes = workspace.nbytes
+    a._tensors = (cache, queries, page_table, lengths, cu_seqlens, out, lse, workspace)
     return a
 
 
-def _norm_rows(t: Tensor, name: str, rows: int, hidden: int, dtype: torch.dtype, device: torch.device) -> tuple[int, int]:
-    _require(t.dim() == 2 and t.size(0) == rows and t.size(1) == hidden and (hidden == 1 or t.stride(1) == 1),
-             f"`{name}` must be [{rows}, {hidden}] with a unit inner stride")
-    _require(t.dtype == dtype and t.device == device, f"`{name}` must be {dtype} on {device}")
-    return t.data_ptr(), t.stride(0)
+def _norm_rows(t: Tensor, name: str, rows: int, hidden: int, dtype: torch.dtype, device: torch.device) -> int:
+    """Row stride of a [rows, hidden] tensor."""
+    row, inner = t.stride() if t.dim() == 2 else (0, 0)
+    if t.shape != (rows, hidden) or (inner != 1 and hidden > 1):
+        raise ValueError(f"`{name}` must be [{rows}, {hidden}] with a unit inner stride")
+    if t.dtype != dtype or t.device != device:
+        raise ValueError(f"`{name}` must be {dtype} on {device}")
+    return row
 
 
 def residual_norm_args(x: Tensor, weight: Tensor, out: Tensor, *, residual: Tensor | None, residual_out: Tensor | None,
                        scales: Tensor | None, eps: float, group: int, flags: int) -> ResidualNormArgs:
     a = ResidualNormArgs()
-    _require(x.dim() == 2 and x.dtype in _NORM_DTYPES, "`x` must be a bf16, fp16 or fp32 [rows, hidden] tensor")
+    dtype, device = x.dtype, x.device
+    if x.dim() != 2 or dtype not in _NORM_DTYPES:
+        raise ValueError("`x` must be a bf16, fp16 or fp32 [rows, hidden] tensor")
     rows, hidden = x.shape
-    a.rows, a.hidden, a.dtype, a.group, a.flags, a.eps = rows, hidden, _NORM_DTYPES[x.dtype], group, flags, eps
-    a.x, a.x_stride = _norm_rows(x, "x", rows, hidden, x.dtype, x.device)
-    _require(weight.dim() == 1 and weight.size(0) == hidden and weight.dtype == x.dtype and weight.device == x.device
-             and (hidden == 1 or weight.stride(0) == 1), f"`weight` must be a contiguous {x.dtype} vector of {hidden} entries on {x.device}")
+    a.rows = rows
+    a.hidden = hidden
+    a.dtype = a.out_dtype = _NORM_DTYPES[dtype]
+    a.group = group
+    a.flags = flags
+    a.eps = eps
+    a.x_stride = _norm_rows(x, "x", rows, hidden, dtype, device)
+    a.x = x.data_ptr()
+    if weight.shape != (hidden,) or weight.dtype != dtype or weight.device != device or (hidden > 1 and weight.stride(0) != 1):
+        raise ValueError(f"`weight` must be a contiguous {dtype} vector of {hidden} entries on {device}")
     a.weight = weight.data_ptr()
     if residual is not None:
-        a.residual, a.residual_stride = _norm_rows(residual, "residual", rows, hidden, x.dtype, x.device)
+        a.residual_stride = _norm_rows(residual, "residual", rows, hidden, dtype, device)
+        a.residual = residual.data_ptr()
     if residual_out is not None:
-        a.residual_out, a.residual_out_stride = _norm_rows(residual_out, "residual_out", rows, hidden, x.dtype, x.device)
-    _require(out.dtype in (x.dtype, E4M3), "`out` must have the dtype of `x`, or be float8_e4m3fn")
-    a.out_dtype = DT_E4M3 if out.dtype == E4M3 else a.dtype
-    a.out, a.out_stride = _norm_rows(out, "out", rows, hidden, out.dtype, x.device)
-    if out.dtype == E4M3:
+        a.residual_out_stride = _norm_rows(residual_out, "residual_out", rows, hidden, dtype, device)
+        a.residual_out = residual_out.data_ptr()
+    out_dtype = out.dtype
+    if out_dtype != dtype and out_dtype != E4M3:
+        raise ValueError("`out` must have the dtype of `x`, or be float8_e4m3fn")
+    a.out_stride = _norm_rows(out, "out", rows, hidden, out_dtype, device)
+    a.out = out.data_ptr()
+    if out_dtype == E4M3:
+        a.out_dtype = DT_E4M3
         groups = -(-hidden // group) if group else 1
-        _require(scales is not None and scales.dtype == F32 and scales.shape == (rows, groups) and scales.is_contiguous()
-                 and scales.device == x.device, f"`scales` must be a contiguous fp32 [{rows}, {groups}] tensor on {x.device}")
+        if scales is None or scales.dtype != F32 or scales.shape != (rows, groups) or not scales.is_contiguous() or scales.device != device:
+            raise ValueError(f"`scales` must be a contiguous fp32 [{rows}, {groups}] tensor on {device}")
         a.scales = scales.data_ptr()
-    _keep(a, x, weight, out, residual, residual_out, scales)
+    a._tensors = (x, weight, out, residual, residual_out, scales)
     return a
 
 
@@ -614,8 +661,14 @@ def paged_attention_workspace_bytes() -> int:
 
 def _launch(name: str, args, device: torch.device) -> None:
     lib = _abi.load_library()
-    with torch.cuda.device(device):
-        _abi.check(getattr(lib, name)(ctypes.byref(args), ctypes.c_void_p(_stream(device))), lib)
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = getattr(lib, name)(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            status = getattr(lib, name)(ctypes.byref(args), _stream(device))
+    if status:
+        _abi.check(status, lib)
 
 
 def launch_cache_append(args: CacheAppendArgs, device: torch.device) -> None:
