@@ -11,9 +11,10 @@ constexpr int MAX_WARPS = MAX_CTAS * WARPS;
 constexpr int PART_FLOATS = 4096;          // a partial result: 8 NT query rows x head_dim at most
 constexpr int PART_ROWS = 32;
 
-// Partial results: slots [0, 2 MAX_WARPS) hold what a warp has of the first and the last unit of its
-// share, slots [2 MAX_WARPS, 2 MAX_WARPS + 2 MAX_CTAS) what a CTA has of its own.
-constexpr int SLOTS = 2 * MAX_WARPS + 2 * MAX_CTAS;
+// Partial results: MAX_WARPS slots for what a warp has of the first unit of its share, where others
+// follow it; then 2 MAX_CTAS for what a CTA has of units that it shares, and 2 MAX_CTAS for sets of
+// CTAs.
+constexpr int SLOTS = MAX_WARPS + 4 * MAX_CTAS;
 struct AttentionWorkspace {
   uint32_t* error;
   uint32_t* tickets;  // [2][2 * MAX_CTAS], zero between calls
@@ -39,7 +40,8 @@ struct AttentionLaunch {
   int window;              // 0 where no request is longer than it
   int each;                // new tokens a request has, without cu_seqlens
   int most;                // new tokens a request has at most, as far as the host knows
-  int direct;              // 0: balanced shares; else one CTA for each of this many row tiles a unit
+  int direct;              // 0: balanced shares; else this many row tiles a (request, kv head) at once
+  int unit_warps;          // warps of each then: 1, or 4 to 32 (a cluster of CTAs)
 };
 
 // The kernel for the types of a call (one translation unit each).

@@ -14,8 +14,9 @@
 //   one a warp, whatever the lengths: a warp finds its place with a scan over `lengths`, and streams
 //   its tiles through its own ring of asynchronous 16-byte copies, which runs ahead across units. No
 //   block barrier until the end.
-// - Where no unit can be long (the page table's width says so), a CTA takes one unit instead, its
-//   warps a quarter each: no scan and nothing to join outside the CTA.
+// - Where no unit can be long (the page table's width says so), a fixed number of warps takes each
+//   unit instead, one warp to a cluster of eight CTAs: no scan, and parts are joined through the
+//   cluster's shared memory.
 // - A unit inside one warp's share goes straight to the output. One that several warps share is
 //   joined in the order of its keys, first by the CTA (through shared memory), then by the last CTA
 //   to arrive (by the square root of their number at a time, where many share it), through the
@@ -44,7 +45,8 @@ constexpr int NT_THREADS = 32 * WARPS;
 constexpr int QUEUE = 8;   // pieces a warp's copies may be ahead of its products
 constexpr int START = 3;   // cost of a unit beside its tiles, in tiles
 constexpr int LEAST = 4;   // cost of a warp's share at least
-constexpr int DIRECT_TILES = 64;  // longest unit that one CTA takes alone
+constexpr int DIRECT_TILES = 16;   // tiles of a warp at most where each unit has its own warps
+constexpr int DIRECT_CTAS = 1184;  // and CTAs of such a launch
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr unsigned ALL = 0xffffffffu;
@@ -58,6 +60,27 @@ __device__ __forceinline__ float4 load_part(const float4* p) {
   float4 v;
   asm volatile("ld.volatile.global.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
   return v;
+}
+
+// the same from either this CTA's shared memory or global memory
+__device__ __forceinline__ float4 load_near(const float4* p) {
+  float4 v;
+  asm volatile("ld.volatile.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+// and from shared memory of CTA `rank` of the cluster, at this CTA's address `at`
+__device__ __forceinline__ float4 load_cluster(uint32_t at, int rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .u32 r;\n\t"
+      "mapa.shared::cluster.u32 r, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [r];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(at), "r"(rank));
+  return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
 // 2^x; 0 for -infinity
@@ -271,7 +294,8 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
   __shared__ Piece shared_piece[WARPS][2];
   __shared__ int shared_live[WARPS][2];  // 1: in the workspace, 2: in the ring
   __shared__ alignas(16) float2 ring_stats[WARPS][PART_ROWS];
-  __shared__ int arrived_last[2 * WARPS];
+  __shared__ alignas(16) float2 cta_stats[PART_ROWS];  // of a unit's parts in this CTA, joined
+  __shared__ uint32_t arrived_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;  // fragment row, and pair of columns
   const SonicSequences& seq = p.a.sequences;
@@ -300,9 +324,10 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
     from = p.window ? max(first - p.window + 1, 0) : 0;
     to = last + 1;
   };
-  // zeros for the query rows of a request without a visible key: heads [head, head + n) of its tokens
-  const auto store_zeros = [&](const Request& q, int head, int n) {
-    for (int i = tid; i < q.new_tokens * n * (D / 4); i += NT_THREADS) {
+  // zeros for the query rows of a request without a visible key: heads [head, head + n) of its tokens,
+  // by threads `thread`, `thread` + `threads`, ...
+  const auto store_zeros = [&](const Request& q, int head, int n, int thread, int threads) {
+    for (int i = thread; i < q.new_tokens * n * (D / 4); i += threads) {
       const int d = i % (D / 4) * 4, h = head + i / (D / 4) % n, row = q.first_row + i / (D / 4) / n;
       A* out = static_cast<A*>(p.a.out) + (int64_t)row * p.a.out_token_stride + (int64_t)h * p.a.out_head_stride + d;
       *reinterpret_cast<uint2*>(out) = make_uint2(0, 0);
@@ -312,19 +337,25 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
 
   // ---- what this CTA does ----
   Request q{};                                   // the request that the copies' side is in
-  int b = 0, direct_head = 0, direct_tile = 0;
+  int b = 0, direct_head = 0, direct_tile = 0, direct_part = 0;
   uint32_t share = 0, cta_begin = 0, cta_end = 0, base = 0;
   bool any_empty = false;
   const auto unit_cost = [](const Request& r) { return r.tiles > 0 ? (uint32_t)r.tiles + START : 0u; };
   if (p.direct) {
-    // one (request, head) and every p.direct'th row tile of it
-    const int index = blockIdx.x / p.direct;
-    direct_tile = blockIdx.x - index * p.direct;
+    // one (request, head) and every p.direct'th row tile of it, for unit_warps warps
+    const int ctas = p.unit_warps / WARPS;
+    int index = ctas ? blockIdx.x / ctas : blockIdx.x * WARPS + warp;
+    direct_part = ctas ? (blockIdx.x - index * ctas) * WARPS + warp : 0;
+    const int tile_of = index;
+    index /= p.direct;
+    direct_tile = tile_of - index * p.direct;
     b = index / heads;
     direct_head = index - b * heads;
+    if (b >= seq.requests) return;
     q = read_request<S>(p, b);
     if (q.tiles == 0) {
-      if (direct_tile == 0) store_zeros(q, direct_head * p.group, p.group);
+      if (direct_tile == 0)
+        store_zeros(q, direct_head * p.group, p.group, direct_part * 32 + lane, p.unit_warps * 32);
       return;
     }
     if (direct_tile >= q.row_tiles) return;
@@ -374,7 +405,7 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
     if (any_empty)
       for (int i = blockIdx.x; i < seq.requests; i += S::CTAS) {
         const Request r = read_request<S>(p, i);
-        if (r.tiles == 0) store_zeros(r, 0, p.a.q_heads);
+        if (r.tiles == 0) store_zeros(r, 0, p.a.q_heads, tid, NT_THREADS);
       }
     if (cta_begin >= cta_end) return;
     q = place[warp].q;
@@ -399,9 +430,12 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
   while (true) {  // once, or in direct mode once a row tile
     // ---- the copies' side: runs STAGES - 1 tiles ahead ----
     int queued = 0, left = 0, key = 0, from = 0, to = 0, stage_in = 0;
-    // Pages of the tiles ahead, asked for a step before they are needed. Runs of keys: lane l holds
-    // the page of run l from the batch's first on; else of key_lane in the next tile.
+    // Pages of the tiles ahead, asked for a step before they are needed. Runs of keys: lane l holds the
+    // page of run l from the batch's first on, from its first use also where the run lies; else of
+    // key_lane in the next tile.
     int pages = 0, batch = 0;
+    int64_t run_at = 0, run_scale = 0;
+    uint32_t runs_there = 0;
     bool ready = false;
     int64_t head_at = 0, scale_head_at = 0;
     const int32_t* table = nullptr;
@@ -432,7 +466,7 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
       table = seq.page_table + (int64_t)b * seq.table_stride;
     };
     if (p.direct) {
-      const int each = (q.tiles + WARPS - 1) / WARPS, tile = warp * each;
+      const int each = (q.tiles + p.unit_warps - 1) / p.unit_warps, tile = direct_part * each;
       if (tile < q.tiles) enter(direct_head, direct_tile, tile, min(each, q.tiles - tile));
     } else if (begin < end) {
       cost = unit_cost(q);
@@ -449,27 +483,41 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
       if (ready) {
         const uint32_t stage = ring + (uint32_t)stage_in * S::STAGE;
         stage_in = stage_in + 1 == S::STAGES ? 0 : stage_in + 1;
-        const int k = key + key_lane;
-        const int page = key_span ? __shfl_sync(ALL, pages, batch + (whole ? 0 : lane >> 4 & MK - 1)) : pages;
-        batch += whole ? 1 : MK;
-        const bool wanted = k + key_span >= from && k < to;
-        const bool there = wanted && (uint32_t)page < (uint32_t)cache.pages;
-        if (wanted && !there) atomicOr(p.ws.error, (uint32_t)SONIC_DEVICE_ERR_PAGE);
-        const int slot = p.page_shift >= 0 ? k & (cache.page_size - 1) : k % cache.page_size;
-        int64_t at = there ? page * cache.page_stride + head_at + slot * cache.slot_stride : 0;
+        // where key_lane of the tile lies, and whether its page is in the cache
+        const auto resolve = [&](int k, int64_t& at, int64_t& scale) {
+          const bool wanted = k + key_span >= from && k < to;
+          const bool there = wanted && (uint32_t)pages < (uint32_t)cache.pages;
+          if (wanted && !there) atomicOr(p.ws.error, (uint32_t)SONIC_DEVICE_ERR_PAGE);
+          const int slot = p.page_shift >= 0 ? k & (cache.page_size - 1) : k % cache.page_size;
+          at = there ? (pages * cache.page_stride + head_at + slot * cache.slot_stride) * (Q8 ? 1 : 2) : 0;
+          if constexpr (Q8) scale = there ? pages * cache.scale_page_stride + scale_head_at + slot : 0;
+          return there;
+        };
+        int64_t at, scale_at = 0;
+        bool there;
+        if (key_span) {
+          if (batch == 0) runs_there = __ballot_sync(ALL, resolve(key + lane * (key_span + 1), run_at, run_scale));
+          const int run = batch + (whole ? 0 : (lane >> 4) & (MK - 1));
+          at = __shfl_sync(ALL, run_at, run);
+          if constexpr (Q8) scale_at = __shfl_sync(ALL, run_scale, run);
+          there = (runs_there >> run) & 1;
+          batch += whole ? 1 : MK;
+        } else {
+          there = resolve(key + key_lane, at, scale_at);
+        }
         const bool all = key >= from && key + KT <= to;
         if (whole && all && there) {
-          const char* src = static_cast<const char*>(cache.keys) + at * (Q8 ? 1 : 2) + lane * 16;
+          const char* src = static_cast<const char*>(cache.keys) + at + lane * 16;
           const uint32_t kd = stage + key_to, vd = stage + value_to;
 #pragma unroll
           for (int i = 0; i < S::COPIES; ++i) {
             copy16((kd ^ S::key_xor(i)) + i * 512, src + i * 512);
             copy16((vd ^ S::value_xor(i)) + i * 512, src + value_delta + i * 512);
           }
-        } else if (MK == 2 && p.packed && !whole && all && __all_sync(ALL, there)) {
+        } else if (MK == 2 && key_span && !whole && all && __all_sync(ALL, there)) {
           const char* src[MK];
 #pragma unroll
-          for (int h = 0; h < MK; ++h) src[h] = static_cast<const char*>(cache.keys) + __shfl_sync(ALL, at, h * 16) * (Q8 ? 1 : 2) + lane * 16;
+          for (int h = 0; h < MK; ++h) src[h] = static_cast<const char*>(cache.keys) + __shfl_sync(ALL, at, h * 16) + lane * 16;
           const uint32_t kd = stage + key_to, vd = stage + value_to;
 #pragma unroll
           for (int i = 0; i < S::COPIES; ++i) {
@@ -478,16 +526,16 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
             copy16((vd ^ S::value_xor(i)) + i * 512, from16 + value_delta);
           }
         } else {
-          // row by row: a lane's key row, or the run that it belongs to
-          if (key_span) at += (int64_t)((lane & (KT - 1)) - key_lane) * cache.slot_stride;
-          const bool row_there = there && key + (lane & (KT - 1)) >= from && key + (lane & (KT - 1)) < to;
-          const uint32_t rows = __ballot_sync(ALL, row_there);
+          // row by row: lane r's address is that of key r
+          const int r_lane = lane & (KT - 1);
+          const int64_t row_at = key_span ? at + (int64_t)(r_lane - key_lane) * cache.slot_stride * (Q8 ? 1 : 2) : at;
+          const uint32_t rows = __ballot_sync(ALL, there && key + r_lane >= from && key + r_lane < to);
 #pragma unroll 4
           for (int i = 0; i < S::COPIES; ++i) {
             const int r = i * S::RPI + row_lane;
-            const int64_t row_at = __shfl_sync(ALL, at, r);
+            const int64_t bytes = __shfl_sync(ALL, row_at, r);
             const bool live = (rows >> r) & 1;
-            const char* src = static_cast<const char*>(cache.keys) + (live ? row_at * (Q8 ? 1 : 2) + piece_lane * 16 : 0);
+            const char* src = static_cast<const char*>(cache.keys) + (live ? bytes + piece_lane * 16 : 0);
             copy16(stage + S::key_at(r, piece_lane), src, live);
             copy16(stage + S::TILE + S::value_at(r, piece_lane), live ? src + value_delta : src, live);
           }
@@ -496,7 +544,7 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
           // lane r copies the scales of key r
           if (lane < KT) {
             const bool live = there && key + lane >= from && key + lane < to;
-            const int64_t sat = live ? page * cache.scale_page_stride + scale_head_at + slot + (key_span ? lane - key_lane : 0) : 0;
+            const int64_t sat = live ? scale_at + (key_span ? lane - key_lane : 0) : 0;
             copy4(stage + 2 * S::TILE + lane * 4, cache.key_scales + sat, live);
             copy4(stage + 2 * S::TILE + KT * 4 + lane * 4, cache.value_scales + sat, live);
           }
@@ -902,6 +950,29 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
       }
     };
 
+    // Row tile j of 8 query rows (from n8 on) into the output; to0 and to1 are the rows that the lane
+    // writes: query row g, or with codes 2t and 2t + 1.
+    const auto store_rows = [&](const Piece& x, int n8, A*& to0, A*& to1) {
+      const int r0 = n8 + (Q8 ? 2 * t : g);
+      to0 = r0 < x.rows ? out_row(x, r0) : nullptr;
+      to1 = Q8 && r0 + 1 < x.rows ? out_row(x, r0 + 1) : nullptr;
+    };
+    const auto store_tile = [&](A* to0, A* to1, int j, const float4& v, float inv0, float inv1) {
+      if constexpr (!Q8) {
+        // pairs of queries a lane -> pairs of dimensions a lane
+        const uint32_t x = transpose8(Pair<A>::pack(v.x * inv0, v.y * inv1));
+        const uint32_t y = transpose8(Pair<A>::pack(v.z * inv0, v.w * inv1));
+        if (to0) {
+          *reinterpret_cast<uint32_t*>(to0 + 16 * j + 2 * t) = x;
+          *reinterpret_cast<uint32_t*>(to0 + 16 * j + 8 + 2 * t) = y;
+        }
+      } else {
+        const int d = S::dimension(j, g);
+        if (to0) *reinterpret_cast<uint32_t*>(to0 + d) = Pair<A>::pack(v.x * inv0, v.z * inv0);
+        if (to1) *reinterpret_cast<uint32_t*>(to1 + d) = Pair<A>::pack(v.y * inv1, v.w * inv1);
+      }
+    };
+
     const auto end_piece = [&]() {
       // the columns' sums over the lanes that share them
 #pragma unroll
@@ -924,36 +995,15 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
             inv[c] = one_over(sum[n][c]);
             if (g == 0 && n * 8 + 2 * t + c < u.rows) store_lse(u, n * 8 + 2 * t + c, ref[n][c], sum[n][c]);
           }
-          if constexpr (!Q8) {
-            // pairs of queries a lane -> pairs of dimensions a lane
-            A* const out = n * 8 + g < u.rows ? out_row(u, n * 8 + g) : nullptr;
+          A *to0, *to1;
+          store_rows(u, n * 8, to0, to1);
 #pragma unroll
-            for (int j = 0; j < DT; ++j) {
-              const uint32_t x = transpose8(Pair<A>::pack(o[j][n][0] * inv[0], o[j][n][1] * inv[1]));
-              const uint32_t y = transpose8(Pair<A>::pack(o[j][n][2] * inv[0], o[j][n][3] * inv[1]));
-              if (out) {
-                *reinterpret_cast<uint32_t*>(out + 16 * j + 2 * t) = x;
-                *reinterpret_cast<uint32_t*>(out + 16 * j + 8 + 2 * t) = y;
-              }
-            }
-          } else {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              if (n * 8 + 2 * t + c >= u.rows) continue;
-              A* const out = out_row(u, n * 8 + 2 * t + c);
-              // row tiles j, j + 1 are 4 consecutive dimensions
-#pragma unroll
-              for (int j = 0; j < DT; j += 2)
-                *reinterpret_cast<uint2*>(out + S::dimension(j, g)) =
-                    make_uint2(Pair<A>::pack(o[j][n][c] * inv[c], o[j][n][2 + c] * inv[c]),
-                               Pair<A>::pack(o[j + 1][n][c] * inv[c], o[j + 1][n][2 + c] * inv[c]));
-            }
-          }
+          for (int j = 0; j < DT; ++j) store_tile(to0, to1, j, make_float4(o[j][n][0], o[j][n][1], o[j][n][2], o[j][n][3]), inv[0], inv[1]);
         }
       } else {
         const int which = taken == 1 ? 0 : 1;  // the share's first piece, or its last
         const bool final = taken == queued && !ready;
-        const size_t slot = 2 * (warp0 + warp) + which;
+        const size_t slot = warp0 + warp;
         if (final) {
           copies_wait<0>();
           __syncwarp();  // the ring is free
@@ -998,6 +1048,119 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
     copies_wait<0>();
 
     // ---- units that several warps share ----
+    // Join n_parts parts of piece x, in order: row tiles j0, j0 + step, ... (J at most), P parts' loads in
+    // flight at once. stats(k, i) and values(k, i) give float4 i of part k; into the output, or to
+    // `stats_to` and `values_to`.
+    const auto join = [&](auto jc, auto pc, const Piece& x, int n_parts, int j0, int step, auto&& stats, auto&& values, bool out,
+                          float4* stats_to, float4* values_to) {
+      constexpr int J = decltype(jc)::value, P = decltype(pc)::value;
+#pragma unroll 1
+      for (int n = 0; n < NT && n * 8 < x.rows; ++n) {
+        const int col = n * 8 + 2 * t;
+        const bool live = col < x.rows;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+        float4 v[J];
+#pragma unroll
+        for (int i = 0; i < J; ++i) v[i] = make_float4(0, 0, 0, 0);
+#pragma unroll 1
+        for (int k0 = 0; k0 < n_parts; k0 += P) {
+          float4 st[P], y[P][J];
+#pragma unroll
+          for (int k = 0; k < P; ++k) {
+            st[k] = make_float4(-INFINITY, 0, -INFINITY, 0);
+            const bool there = live && k0 + k < n_parts;
+            if (there) st[k] = stats(k0 + k, col / 2);
+#pragma unroll
+            for (int i = 0; i < J; ++i) {
+              y[k][i] = make_float4(0, 0, 0, 0);
+              if (there && j0 + i * step < DT) y[k][i] = values(k0 + k, ((j0 + i * step) * NT + n) * 32 + lane);
+            }
+          }
+          float t0 = m0, t1 = m1;
+#pragma unroll
+          for (int k = 0; k < P; ++k) t0 = fmaxf(t0, st[k].x), t1 = fmaxf(t1, st[k].z);
+          const float a0 = m0 == -INFINITY ? 0.0f : exp2_fast(m0 - t0), a1 = m1 == -INFINITY ? 0.0f : exp2_fast(m1 - t1);
+          m0 = t0, m1 = t1, l0 *= a0, l1 *= a1;
+#pragma unroll
+          for (int i = 0; i < J; ++i) v[i].x *= a0, v[i].z *= a0, v[i].y *= a1, v[i].w *= a1;
+#pragma unroll
+          for (int k = 0; k < P; ++k) {
+            const float f0 = st[k].x == -INFINITY ? 0.0f : exp2_fast(st[k].x - m0), f1 = st[k].z == -INFINITY ? 0.0f : exp2_fast(st[k].z - m1);
+            l0 = fmaf(st[k].y, f0, l0), l1 = fmaf(st[k].w, f1, l1);
+#pragma unroll
+            for (int i = 0; i < J; ++i) {
+              v[i].x = fmaf(f0, y[k][i].x, v[i].x), v[i].z = fmaf(f0, y[k][i].z, v[i].z);
+              v[i].y = fmaf(f1, y[k][i].y, v[i].y), v[i].w = fmaf(f1, y[k][i].w, v[i].w);
+            }
+          }
+        }
+        const bool first = j0 == 0 && g == 0 && live;  // this lane also writes the columns' statistics
+        if (out) {
+          A *to0, *to1;
+          store_rows(x, n * 8, to0, to1);
+          const float inv0 = one_over(l0), inv1 = one_over(l1);
+#pragma unroll
+          for (int i = 0; i < J; ++i)
+            if (j0 + i * step < DT) store_tile(to0, to1, j0 + i * step, v[i], inv0, inv1);
+          if (first) {
+            store_lse(x, col, m0, l0);
+            if (col + 1 < x.rows) store_lse(x, col + 1, m1, l1);
+          }
+        } else if (live) {
+#pragma unroll
+          for (int i = 0; i < J; ++i)
+            if (j0 + i * step < DT) values_to[((j0 + i * step) * NT + n) * 32 + lane] = v[i];
+          if (first) stats_to[col / 2] = make_float4(m0, l0, m1, l1);
+        }
+      }
+    };
+    using PerWarp = std::integral_constant<int, (DT + WARPS - 1) / WARPS>;  // row tiles of a warp of the CTA
+    using PerClusterWarp = std::integral_constant<int, imax(1, DT / 8)>;  // of 8 warps or more
+    using Few = std::integral_constant<int, WARPS>;
+    using Many = std::integral_constant<int, 8>;
+
+    if (p.direct) {
+      const int next_tile = direct_tile + p.direct;
+      if (p.unit_warps >= WARPS) {
+        // a unit's parts lie in the rings of consecutive warps: joined in each CTA, then in the cluster
+        const int each = (q.tiles + p.unit_warps - 1) / p.unit_warps, n = (q.tiles + each - 1) / each;
+        const int ctas = p.unit_warps / WARPS, rank = direct_part / WARPS;
+        Piece x;
+        x.head = direct_head;
+        x.row0 = direct_tile * S::ROWS;
+        x.rows = min(S::ROWS, q.new_tokens * p.group - x.row0);
+        x.first_row = q.first_row;
+        __syncthreads();
+        const int here = min(n - rank * WARPS, WARPS);
+        const uint32_t values_at = shared_address(smem), stats_at = shared_address(ring_stats);
+        const auto load_here = [](uint32_t at) {
+          const uint4 v = load_shared16(at);
+          return make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+        };
+        if (n > 1 && here > 0)
+          join(
+              PerWarp{}, Few{}, x, here, warp, WARPS, [&](int k, int i) { return load_here(stats_at + k * PART_ROWS * 8 + i * 16); },
+              [&](int k, int i) { return load_here(values_at + k * S::WARP_BYTES + i * 16); }, ctas == 1,
+              reinterpret_cast<float4*>(cta_stats), reinterpret_cast<float4*>(smem));  // (each thread reads what it overwrites)
+        if (ctas > 1) {
+          cluster_barrier();
+          if (n > 1) {
+            const uint32_t cta_stats_at = shared_address(cta_stats);
+            join(
+                PerClusterWarp{}, Many{}, x, (n + WARPS - 1) / WARPS, direct_part, p.unit_warps,
+                [&](int k, int i) { return load_cluster(cta_stats_at + i * 16, k); },
+                [&](int k, int i) { return load_cluster(values_at + i * 16, k); }, true, nullptr, nullptr);
+          }
+          cluster_barrier();  // nobody's shared memory goes before all have read it
+        } else if (next_tile < q.row_tiles) {
+          __syncthreads();
+        }
+      }
+      direct_tile = next_tile;
+      if (direct_tile >= q.row_tiles) return;
+      continue;
+    }
+
     __syncthreads();
     // Every warp looks at the CTA's pieces, lane x at piece (w, which) = (x / 2, x % 2): is it the
     // CTA's first of its unit, and how many consecutive warps have a part?
@@ -1018,174 +1181,91 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
         const uint32_t unit_there = __shfl_sync(ALL, part_unit, 2 * from);
         if (parts == k && from < WARPS && live && unit_there == part_unit && tile0 > 0 && part_last < part_tiles) parts = k + 1, part_last = last;
       }
+      if (lane >= 2 * WARPS) parts = 0;
     }
-    const bool crosses = __any_sync(ALL, parts > 0 && (part_tile0 > 0 || part_last < part_tiles));
+    const bool mine_crosses = parts > 0 && (part_tile0 > 0 || part_last < part_tiles);
+    const uint32_t groups = __ballot_sync(ALL, parts > 0), crossing = __ballot_sync(ALL, mine_crosses);
+    const uint32_t in_ring = __ballot_sync(ALL, part_live == 2);
     // The CTAs that have a part of a unit, c0 and the `ctas` from it on; and their slots: 0 is for the
     // unit that an earlier CTA began, 1 for one that the CTA begins.
-    const auto find_ctas = [&](const Piece& x, int& c0, int& ctas) {
-      const auto part_before = [&](uint32_t index) { return cut(index * share, index, x.unit, x.unit_tiles); };
-      uint32_t g0 = x.unit / share, g1 = (x.unit + x.unit_tiles + START - 1) / share;
+    int c0 = 0, ctas = 0;  // of piece `lane`
+    if (mine_crosses) {
+      const auto part_before = [&](uint32_t index) { return cut(index * share, index, part_unit, part_tiles); };
+      uint32_t g0 = part_unit / share, g1 = (part_unit + part_tiles + START - 1) / share;
       while (part_before(g0 + 1) == 0) ++g0;
-      while (part_before(g1) == x.unit_tiles) --g1;
+      while (part_before(g1) == part_tiles) --g1;
       c0 = g0 / WARPS;
       ctas = (int)(g1 / WARPS) - c0 + 1;
-    };
-    const auto cta_slot = [](int c0, int k) { return (size_t)(2 * MAX_WARPS + (k == 0 ? 2 * c0 + 1 : 2 * (c0 + k))); };
-    // Join n parts of piece x: part k's accumulators and statistics lie where `where` says. Thread
-    // (warp, lane) takes row tiles warp, warp + 4, ... of its query columns 2t and 2t + 1. Into the
-    // output, or into slot `slot_to` of the workspace.
-    const auto join = [&](const Piece& x, int n_parts, auto&& load_stats, auto&& load_values, bool out, size_t slot_to) {
-#pragma unroll 1
-      for (int n = 0; n < NT; ++n) {
-        const int col = n * 8 + 2 * t;
-        if (col >= x.rows) break;
-        const bool second = col + 1 < x.rows;
-        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-#pragma unroll 4
-        for (int k = 0; k < n_parts; ++k) {
-          const float4 st = load_stats(k, col / 2);
-          m0 = fmaxf(m0, st.x), m1 = fmaxf(m1, st.z);
-        }
-        float4 v[(DT + WARPS - 1) / WARPS];
-#pragma unroll
-        for (int j = 0; j < (DT + WARPS - 1) / WARPS; ++j) v[j] = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-        for (int k = 0; k < n_parts; ++k) {
-          const float4 st = load_stats(k, col / 2);
-          const float f0 = st.x == -INFINITY ? 0.0f : exp2_fast(st.x - m0), f1 = st.z == -INFINITY ? 0.0f : exp2_fast(st.z - m1);
-          l0 = fmaf(st.y, f0, l0), l1 = fmaf(st.w, f1, l1);
-#pragma unroll
-          for (int j = 0; j < (DT + WARPS - 1) / WARPS; ++j) {
-            if (DT % WARPS != 0 && warp + j * WARPS >= DT) break;
-            const float4 y = load_values(k, ((warp + j * WARPS) * NT + n) * 32 + lane);
-            v[j].x = fmaf(f0, y.x, v[j].x), v[j].z = fmaf(f0, y.z, v[j].z);
-            v[j].y = fmaf(f1, y.y, v[j].y), v[j].w = fmaf(f1, y.w, v[j].w);
-          }
-        }
-        if (!second) l1 = 0.0f, m1 = -INFINITY;  // (nobody wrote that column)
-        if (!out) {
-#pragma unroll
-          for (int j = 0; j < (DT + WARPS - 1) / WARPS; ++j)
-            if (DT % WARPS == 0 || warp + j * WARPS < DT) p.ws.parts[slot_to * (PART_FLOATS / 4) + ((warp + j * WARPS) * NT + n) * 32 + lane] = v[j];
-          if (warp == 0 && g == 0) reinterpret_cast<float4*>(p.ws.stats + slot_to * PART_ROWS)[col / 2] = make_float4(m0, l0, m1, l1);
-          continue;
-        }
-        if (warp == 0 && g == 0) {
-          store_lse(x, col, m0, l0);
-          if (second) store_lse(x, col + 1, m1, l1);
-        }
-        const float inv0 = one_over(l0), inv1 = one_over(l1);
-        A* const out0 = out_row(x, col);
-        A* const out1 = second ? out_row(x, col + 1) : nullptr;
-#pragma unroll
-        for (int j = 0; j < (DT + WARPS - 1) / WARPS; ++j) {
-          if (DT % WARPS != 0 && warp + j * WARPS >= DT) break;
-          const int d0 = S::dimension(warp + j * WARPS, g), d1 = S::dimension(warp + j * WARPS, g + 8);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            A* const to = c ? out1 : out0;
-            if (!to) continue;
-            const uint32_t pair = c ? Pair<A>::pack(v[j].y * inv1, v[j].w * inv1) : Pair<A>::pack(v[j].x * inv0, v[j].z * inv0);
-            if constexpr (Q8) {
-              *reinterpret_cast<uint32_t*>(to + d0) = pair;
-            } else {
-              reinterpret_cast<uint16_t*>(to)[d0] = (uint16_t)pair;
-              reinterpret_cast<uint16_t*>(to)[d1] = (uint16_t)(pair >> 16);
-            }
-          }
-        }
-      }
-    };
+    }
+    const auto cta_slot = [](int c, int k) { return (size_t)(MAX_WARPS + (k == 0 ? 2 * c + 1 : 2 * (c + k))); };
 
     // -- inside the CTA --
 #pragma unroll 1
-    for (int x = 0; x < 2 * WARPS; ++x) {
-      const int n = __shfl_sync(ALL, parts, x);
-      if (n == 0) continue;
-      const int w = x >> 1;
-      const Piece first = shared_piece[w][x & 1];
-      const int last = __shfl_sync(ALL, part_last, x);
-      const bool out = first.tile0 == 0 && last == first.unit_tiles;
-      size_t slot_to = 0;
-      if (!out) {
-        int c0, ctas;
-        find_ctas(first, c0, ctas);
-        slot_to = cta_slot(c0, (int)blockIdx.x - c0);
-      }
-      // only a first piece can lie in the workspace: part 0, when it is one
-      const bool ring0 = shared_live[w][x & 1] == 2;
-      bool ring[WARPS];
-#pragma unroll
-      for (int k = 1; k < WARPS; ++k) ring[k] = w + k < WARPS && shared_live[min(w + k, WARPS - 1)][0] == 2;
-      const auto in_ring = [&](int k) { return k == 0 ? ring0 : k == 1 ? ring[1] : k == 2 ? ring[2] : ring[3]; };
-      const auto slot = [&](int k) { return (size_t)(2 * (warp0 + w + k) + (k == 0 ? x & 1 : 0)); };
+    for (uint32_t left_groups = groups; left_groups; left_groups &= left_groups - 1) {
+      const int x = __ffs(left_groups) - 1, w = x >> 1, n = __shfl_sync(ALL, parts, x);
+      const bool out = !((crossing >> x) & 1);
+      const int c = __shfl_sync(ALL, c0, x);
+      // part k lies in warp w + k's ring, or (a first piece that others followed) in the workspace
+      const auto place_of = [&](int k, const float4* ring_at, const float4* slots, size_t slot_size) {
+        const int piece = 2 * (w + k) + (k == 0 ? x & 1 : 0);
+        return (in_ring >> piece) & 1 ? ring_at : slots + (size_t)(warp0 + w + k) * slot_size;
+      };
+      const size_t to = out ? 0 : cta_slot(c, (int)blockIdx.x - c);
       join(
-          first, n,
+          PerWarp{}, Few{}, shared_piece[w][x & 1], n, warp, WARPS,
           [&](int k, int i) {
-            return in_ring(k) ? reinterpret_cast<const float4*>(ring_stats[w + k])[i]
-                              : load_part(reinterpret_cast<const float4*>(p.ws.stats + slot(k) * PART_ROWS) + i);
+            return load_near(place_of(k, reinterpret_cast<const float4*>(ring_stats[w + k]), reinterpret_cast<const float4*>(p.ws.stats), PART_ROWS / 2) + i);
           },
           [&](int k, int i) {
-            return in_ring(k) ? reinterpret_cast<const float4*>(smem + (w + k) * S::WARP_BYTES)[i] : load_part(p.ws.parts + slot(k) * (PART_FLOATS / 4) + i);
+            return load_near(place_of(k, reinterpret_cast<const float4*>(smem + (w + k) * S::WARP_BYTES), p.ws.parts, PART_FLOATS / 4) + i);
           },
-          out, slot_to);
+          out, reinterpret_cast<float4*>(p.ws.stats + to * PART_ROWS), p.ws.parts + to * (PART_FLOATS / 4));
     }
-    if (p.direct) {
-      direct_tile += p.direct;
-      if (direct_tile >= q.row_tiles) return;
-      __syncthreads();
-      if (tid < 2 * WARPS) shared_live[tid >> 1][tid & 1] = 0;
-      __syncthreads();
-      continue;
-    }
-    if (!crosses) return;
+    if (!crossing) return;
 
     // -- units of several CTAs: the last of them to arrive joins their parts, in sets of `size` where
     // there are many, then the sets. A CTA has at most two such units: both arrive together. --
+    int size = max(ctas, 1);
+    if (ctas > 12) {
+      size = 4;
+      while (size * size < ctas) ++size;
+    }
+    const int sets = (ctas + size - 1) / size, set = ((int)blockIdx.x - c0) / size;
+    uint32_t waiting = crossing;  // units whose last arrival at the level before was here
 #pragma unroll 1
-    for (int level = 1; level <= 2; ++level) {
+    for (int level = 1; level <= 2 && waiting; ++level) {
       __threadfence();
       __syncthreads();
-      const auto sets_of = [](int ctas, int& size) {
-        size = ctas;
-        if (ctas > 12) {
-          size = 4;
-          while (size * size < ctas) ++size;
-        }
-        return (ctas + size - 1) / size;
-      };
-      if (tid < 2 * WARPS) {
+      if (warp == 0) {
         int last = 0;
-        if (parts > 0 && (part_tile0 > 0 || part_last < part_tiles) && (level == 1 || arrived_last[tid])) {
-          int c0, ctas, size;
-          find_ctas(shared_piece[tid >> 1][tid & 1], c0, ctas);
-          const int sets = sets_of(ctas, size), set = ((int)blockIdx.x - c0) / size;
+        if ((waiting >> lane) & 1) {
           const int members = level == 1 ? min(size, ctas - set * size) : sets;
-          uint32_t* const ticket = p.ws.tickets + (level - 1) * 2 * MAX_CTAS + cta_slot(c0, level == 1 ? set * size : 0) - 2 * MAX_WARPS;
+          uint32_t* const ticket = p.ws.tickets + (level - 1) * 2 * MAX_CTAS + cta_slot(c0, level == 1 ? set * size : 0) - MAX_WARPS;
           last = level == 1 || sets > 1 ? atomicAdd(ticket, 1u) + 1 == (uint32_t)members : 0;
           if (last) *ticket = 0;
         }
-        arrived_last[tid] = last;
+        const uint32_t arrived = __ballot_sync(ALL, last);
+        if (lane == 0) arrived_last = arrived;
       }
       __syncthreads();
+      waiting = arrived_last;
       __threadfence();
-      bool more = false;
 #pragma unroll 1
-      for (int x = 0; x < 2 * WARPS; ++x) {
-        if (!arrived_last[x]) continue;
-        const Piece first = shared_piece[x >> 1][x & 1];
-        int c0, ctas, size;
-        find_ctas(first, c0, ctas);
-        const int sets = sets_of(ctas, size), set = ((int)blockIdx.x - c0) / size;
-        const bool out = level == 2 || sets == 1;
-        const auto slot = [&](int k) { return cta_slot(c0, level == 1 ? set * size + k : k * size); };
-        more = more || !out;
+      for (uint32_t todo_groups = waiting; todo_groups; todo_groups &= todo_groups - 1) {
+        const int x = __ffs(todo_groups) - 1;
+        const int c = __shfl_sync(ALL, c0, x), n = __shfl_sync(ALL, ctas, x), step = __shfl_sync(ALL, size, x);
+        const int count = __shfl_sync(ALL, sets, x), mine = __shfl_sync(ALL, set, x);
+        const bool out = level == 2 || count == 1;
+        // (a set's result goes to a slot of its own: all of its members are being read)
+        const auto slot = [&](int k) { return level == 1 ? cta_slot(c, mine * step + k) : cta_slot(c, k * step) + 2 * MAX_CTAS; };
+        const size_t to = cta_slot(c, mine * step) + 2 * MAX_CTAS;
         join(
-            first, level == 1 ? min(size, ctas - set * size) : sets,
+            PerWarp{}, Many{}, shared_piece[x >> 1][x & 1], level == 1 ? min(step, n - mine * step) : count, warp, WARPS,
             [&](int k, int i) { return load_part(reinterpret_cast<const float4*>(p.ws.stats + slot(k) * PART_ROWS) + i); },
-            [&](int k, int i) { return load_part(p.ws.parts + slot(k) * (PART_FLOATS / 4) + i); }, out, slot(0));
+            [&](int k, int i) { return load_part(p.ws.parts + slot(k) * (PART_FLOATS / 4) + i); }, out,
+            reinterpret_cast<float4*>(p.ws.stats + to * PART_ROWS), p.ws.parts + to * (PART_FLOATS / 4));
+        if (out) waiting &= ~(1u << x);
       }
-      if (!more) break;
     }
     return;
   }
@@ -1198,20 +1278,27 @@ sonic_status launch_attention(const AttentionLaunch& launch, cudaStream_t stream
   const SonicSequences& s = p.a.sequences;
   const int64_t row_tiles = ((int64_t)p.most * p.group + S::ROWS - 1) / S::ROWS;
   const int64_t units = (int64_t)s.requests * p.a.cache.kv_heads * row_tiles;
-  // one CTA a unit where none has more than 64 tiles (a warp then streams 16 at most): the balanced
-  // shares' scan and joins cost more than the uneven lengths do
+  // A fixed number of warps a unit, as many as leave a warp DIRECT_TILES of the longest possible one,
+  // where that takes no more than DIRECT_CTAS CTAs: the balanced shares' scan and joins cost more
+  // than the uneven lengths do.
   const int64_t tiles = ((p.window ? std::min<int64_t>(p.room, (int64_t)p.window + p.most) : p.room) + S::KT - 1) / S::KT + 1;
-  if (tiles <= DIRECT_TILES && units <= INT32_MAX) {
+  p.unit_warps = 1;
+  while (p.unit_warps < 32 && tiles > (int64_t)DIRECT_TILES * p.unit_warps) p.unit_warps = p.unit_warps == 1 ? WARPS : 2 * p.unit_warps;
+  // few units: more warps each, down to two tiles a warp
+  while (p.unit_warps < 32 && tiles > 2 * p.unit_warps && units * (p.unit_warps == 1 ? WARPS : 2 * p.unit_warps) <= S::CTAS * WARPS)
+    p.unit_warps = p.unit_warps == 1 ? WARPS : 2 * p.unit_warps;
+  const int64_t ctas = (units * p.unit_warps + WARPS - 1) / WARPS;
+  if (tiles <= (int64_t)DIRECT_TILES * p.unit_warps && ctas <= DIRECT_CTAS) {
     p.direct = (int)std::max<int64_t>(1, row_tiles);
-    return launch_status(launch_kernel(attention_kernel<A, Q8, D, NT>, dim3((unsigned)units), dim3(NT_THREADS), S::SMEM, stream,
-                                       p.a.flags & SONIC_FLAG_PDL, p));
+    return launch_status(launch_kernel(attention_kernel<A, Q8, D, NT>, dim3((unsigned)ctas), dim3(NT_THREADS), S::SMEM, stream,
+                                       p.a.flags & SONIC_FLAG_PDL, std::max(1, p.unit_warps / WARPS), p));
   }
   // cost the kernel's 32-bit counters can meet: every page-table row full
   const double most_cost = ((double)p.room / S::KT + 2 + START) * ((double)s.tokens * p.group / S::ROWS + s.requests) * p.a.cache.kv_heads;
   if (most_cost >= 2.0e9) return fail_with(SONIC_ERR_UNSUPPORTED, "the call spans more than 2^32 steps: split it by requests");
   p.direct = 0;
   return launch_status(launch_kernel(attention_kernel<A, Q8, D, NT>, dim3(S::CTAS), dim3(NT_THREADS), S::SMEM, stream,
-                                     p.a.flags & SONIC_FLAG_PDL, p));
+                                     p.a.flags & SONIC_FLAG_PDL, 1, p));
 }
 
 template <typename A, bool Q8>

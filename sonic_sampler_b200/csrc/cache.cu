@@ -242,7 +242,7 @@ extern "C" sonic_status sonic_cache_append(const SonicCacheAppendArgs* a, void* 
   const dim3 grid((a->sequences.tokens + run - 1) / run);
   const bool pdl = a->flags & SONIC_FLAG_PDL;
   const auto go = [&](auto kernel) {
-    return launch_status(launch_kernel(kernel, grid, dim3(NT), 0, (cudaStream_t)stream, pdl, *a, run, log2_of(lanes)));
+    return launch_status(launch_kernel(kernel, grid, dim3(NT), 0, (cudaStream_t)stream, pdl, 1, *a, run, log2_of(lanes)));
   };
   const bool q8 = a->cache.dtype == SONIC_DTYPE_E4M3;
   if (a->dtype == SONIC_DTYPE_BF16) return q8 ? go(append_kernel<__nv_bfloat16, true>) : go(append_kernel<__nv_bfloat16, false>);
@@ -265,7 +265,7 @@ extern "C" sonic_status sonic_cache_gather(const SonicCacheGatherArgs* a, void* 
   const dim3 grid((a->sequences.tokens + run - 1) / run);
   const bool pdl = a->flags & SONIC_FLAG_PDL;
   const auto go = [&](auto kernel) {
-    return launch_status(launch_kernel(kernel, grid, dim3(NT), 0, (cudaStream_t)stream, pdl, *a, run, log2_of(lanes)));
+    return launch_status(launch_kernel(kernel, grid, dim3(NT), 0, (cudaStream_t)stream, pdl, 1, *a, run, log2_of(lanes)));
   };
   if (a->dtype == SONIC_DTYPE_BF16) return q8 ? go(gather_kernel<__nv_bfloat16, true>) : go(gather_kernel<__nv_bfloat16, false>);
   return q8 ? go(gather_kernel<__half, true>) : go(gather_kernel<__half, false>);

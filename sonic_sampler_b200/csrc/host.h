@@ -17,9 +17,10 @@ inline sonic_status launch_status(cudaError_t e) noexcept {
 }
 
 // Launch with `smem` bytes of dynamic shared memory; with `pdl` the kernel may start before the
-// stream's previous kernel has ended (it waits with griddepcontrol.wait before its first access).
+// stream's previous kernel has ended (it waits with griddepcontrol.wait before its first access);
+// `cluster` CTAs form a cluster.
 template <typename Kern, typename... Args>
-cudaError_t launch_kernel(Kern kern, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool pdl,
+cudaError_t launch_kernel(Kern kern, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool pdl, int cluster,
                           const Args&... args) noexcept {
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -30,11 +31,19 @@ cudaError_t launch_kernel(Kern kern, dim3 grid, dim3 block, size_t smem, cudaStr
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
+  cfg.numAttrs = 0;
+  if (pdl) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
 

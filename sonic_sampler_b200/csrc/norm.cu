@@ -245,7 +245,7 @@ sonic_status run(const SonicResidualNormArgs& a, cudaStream_t stream) {
   const int rows = warps == 1 ? std::min(a.rows, 4) : 1;
   const dim3 block(32 * warps, rows), grid((a.rows + rows - 1) / rows);
   const bool pdl = a.flags & SONIC_FLAG_PDL;
-  const auto go = [&](auto kernel) { return launch_status(launch_kernel(kernel, grid, block, 0, stream, pdl, a)); };
+  const auto go = [&](auto kernel) { return launch_status(launch_kernel(kernel, grid, block, 0, stream, pdl, 1, a)); };
   switch (n) {
     case 1: return go(norm_kernel<T, Q8, VEC, 1>);
     case 2: return go(norm_kernel<T, Q8, VEC, 2>);
