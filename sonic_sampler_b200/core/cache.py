@@ -82,11 +82,8 @@ class PagedCache:
         ops._require_cuda(page_table)
         if dtype is None:
             dtype = keys.dtype if keys is not None else torch.bfloat16 if self.keys.dtype == E4M3 else self.keys.dtype
-        shape = (total, self.struct.kv_heads, self.struct.head_dim)
-        keys = self.keys.new_empty(shape, dtype=dtype) if keys is None else keys
-        values = self.keys.new_empty(shape, dtype=dtype) if values is None else values
-        args = ops.cache_gather_args(self.struct, page_table, starts, keys, values, flags=self.flags,
-                                     error=self.errors, device=self.device)
+        args, keys, values = ops.cache_gather_args(self.struct, page_table, starts, total, dtype, keys, values, flags=self.flags,
+                                                   error=self.errors, device=self.device)
         ops.launch_cache_gather(args, self.device)
         return keys, values
 

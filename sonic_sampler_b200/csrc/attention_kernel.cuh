@@ -45,8 +45,6 @@ constexpr int NT_THREADS = 32 * WARPS;
 constexpr int QUEUE = 8;   // pieces a warp's copies may be ahead of its products
 constexpr int START = 3;   // cost of a unit beside its tiles, in tiles
 constexpr int LEAST = 4;   // cost of a warp's share at least
-constexpr int DIRECT_TILES = 16;   // tiles of a warp at most where each unit has its own warps
-constexpr int DIRECT_CTAS = 1184;  // and CTAs of such a launch
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr unsigned ALL = 0xffffffffu;
@@ -1278,17 +1276,24 @@ sonic_status launch_attention(const AttentionLaunch& launch, cudaStream_t stream
   const SonicSequences& s = p.a.sequences;
   const int64_t row_tiles = ((int64_t)p.most * p.group + S::ROWS - 1) / S::ROWS;
   const int64_t units = (int64_t)s.requests * p.a.cache.kv_heads * row_tiles;
-  // A fixed number of warps a unit, as many as leave a warp DIRECT_TILES of the longest possible one,
-  // where that takes no more than DIRECT_CTAS CTAs: the balanced shares' scan and joins cost more
-  // than the uneven lengths do.
+  // A fixed number of warps a unit where that leaves a warp at most 16 tiles of the longest possible
+  // one, in up to two waves of CTAs, or 32 in at least half a wave and at most one: there the balanced
+  // shares' scan and joins cost more than uneven lengths do. (us, fixed against balanced: 37 requests of
+  // 1024 keys, 8 kv heads, bf16: 29 against 36; 64 of up to 1000, 4 queries: 34 against 37; 32 of up to
+  // 4097, 5 queries, which would take 1024 CTAs: 49 against 33.)
   const int64_t tiles = ((p.window ? std::min<int64_t>(p.room, (int64_t)p.window + p.most) : p.room) + S::KT - 1) / S::KT + 1;
+  const auto ctas_of = [&](int warps) { return (units * warps + WARPS - 1) / WARPS; };
+  const auto more = [](int warps) { return warps == 1 ? WARPS : 2 * warps; };
+  const auto fits = [&](int warps) {
+    const int64_t ctas = ctas_of(warps);
+    return (tiles <= 16 * warps && ctas <= 2 * S::CTAS) || (tiles <= 32 * warps && 2 * ctas >= S::CTAS && ctas <= S::CTAS);
+  };
   p.unit_warps = 1;
-  while (p.unit_warps < 32 && tiles > (int64_t)DIRECT_TILES * p.unit_warps) p.unit_warps = p.unit_warps == 1 ? WARPS : 2 * p.unit_warps;
-  // few units: more warps each, down to two tiles a warp
-  while (p.unit_warps < 32 && tiles > 2 * p.unit_warps && units * (p.unit_warps == 1 ? WARPS : 2 * p.unit_warps) <= S::CTAS * WARPS)
-    p.unit_warps = p.unit_warps == 1 ? WARPS : 2 * p.unit_warps;
-  const int64_t ctas = (units * p.unit_warps + WARPS - 1) / WARPS;
-  if (tiles <= (int64_t)DIRECT_TILES * p.unit_warps && ctas <= DIRECT_CTAS) {
+  while (p.unit_warps < 32 && !fits(p.unit_warps)) p.unit_warps = more(p.unit_warps);
+  if (fits(p.unit_warps)) {
+    // few units: more warps each, down to two tiles a warp
+    while (p.unit_warps < 32 && tiles > 2 * p.unit_warps && ctas_of(more(p.unit_warps)) <= S::CTAS) p.unit_warps = more(p.unit_warps);
+    const int64_t ctas = ctas_of(p.unit_warps);
     p.direct = (int)std::max<int64_t>(1, row_tiles);
     return launch_status(launch_kernel(attention_kernel<A, Q8, D, NT>, dim3((unsigned)ctas), dim3(NT_THREADS), S::SMEM, stream,
                                        p.a.flags & SONIC_FLAG_PDL, std::max(1, p.unit_warps / WARPS), p));

@@ -53,17 +53,58 @@ __device__ __forceinline__ Slot find_slot(const SonicPagedCache& c, const SonicS
   return found;
 }
 
-// Each thread moves 8 activations: 16 bytes in; 16 bytes (16-bit cache) or 8 codes out. A row is
-// head_dim / 8 neighbouring lanes (8, 16 or 32), which reduce its largest magnitude by shuffles.
+// Pieces of the run's tokens, `lanes` neighbouring threads a (token, keys or values, head) row: piece
+// i of thread `tid`, of ITEMS a thread at most.
+constexpr int ITEMS = 4;
+
+struct Work {
+  int run;             // tokens a CTA takes
+  int row_shift;       // log2 of the lanes a row has
+  uint32_t per_token;  // rows a token has
+  uint32_t inverse;    // floor(2^32 / per_token) + 1: r / per_token is the high half of r times it
+};
+
+struct Item {
+  bool live;
+  int t, half, head, lane;
+};
+
+__device__ __forceinline__ Item item_of(const Work& w, int i, int count, int heads) {
+  Item x;
+  const uint32_t r = ((blockIdx.y * ITEMS + i) * NT + threadIdx.x) >> w.row_shift;
+  x.lane = threadIdx.x & ((1 << w.row_shift) - 1);
+  x.live = r < count * w.per_token;
+  x.t = __umulhi(r, w.inverse);
+  const int rest = r - x.t * w.per_token;
+  x.half = rest >= heads;
+  x.head = x.half ? rest - heads : rest;
+  return x;
+}
+
+// Each thread moves 8 activations an item: 16 bytes in; 16 bytes (16-bit cache) or 8 codes out. A row
+// is head_dim / 8 neighbouring lanes (8, 16 or 32), which reduce its largest magnitude by shuffles.
+// The activations are asked for before the tokens are looked up, all items' at once: 16000 tokens of 8
+// heads of 128 take XXAPPEND us (one item at a time, after the look-up: 34 us).
 template <typename T, bool Q8>
-__global__ void __launch_bounds__(NT) append_kernel(SonicCacheAppendArgs a, int run, int row_shift) {
+__global__ void __launch_bounds__(NT) append_kernel(SonicCacheAppendArgs a, Work work) {
   __shared__ Slot slots[MAX_RUN];
   grid_dependency_trigger();
-  grid_dependency_wait();
   const SonicSequences& s = a.sequences;
   const SonicPagedCache& c = a.cache;
-  const int first = blockIdx.x * run;
-  const int count = min(run, s.tokens - first);
+  const int first = blockIdx.x * work.run;
+  const int count = min(work.run, s.tokens - first);
+  grid_dependency_wait();
+  uint4 x[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const Item item = item_of(work, i, count, c.kv_heads);
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (item.live) {
+      const int64_t at = item.half ? (first + item.t) * a.value_token_stride + item.head * a.value_head_stride
+                                   : (first + item.t) * a.key_token_stride + item.head * a.key_head_stride;
+      x[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(item.half ? a.values : a.keys) + at + item.lane * 8);
+    }
+  }
   if (threadIdx.x < count) {
     const int row = first + threadIdx.x;
     Slot found;
@@ -79,31 +120,21 @@ __global__ void __launch_bounds__(NT) append_kernel(SonicCacheAppendArgs a, int 
     slots[threadIdx.x] = found;
   }
   __syncthreads();
-  const int lanes = 1 << row_shift;                  // lanes a row
-  const int rows = count * c.kv_heads * 2;           // (token, head, keys / values)
-  const int lane = threadIdx.x & (lanes - 1);
-  // all lanes of a warp make the same number of rounds: the shuffles below are warp-wide
-  const int rounds = (rows * lanes + NT - 1) / NT;
-  for (int i = 0; i < rounds; ++i) {
-    const int r = (i * NT + threadIdx.x) >> row_shift;
-    const bool live = r < rows;
-    const int half = r & 1, head = (r >> 1) % c.kv_heads, t = (r >> 1) / c.kv_heads;
-    uint4 x = make_uint4(0, 0, 0, 0);
+  const int lanes = 1 << work.row_shift;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const Item item = item_of(work, i, count, c.kv_heads);
     Slot slot;
-    if (live) {
-      slot = slots[t];
-      const int64_t at = half ? (first + t) * a.value_token_stride + head * a.value_head_stride
-                              : (first + t) * a.key_token_stride + head * a.key_head_stride;
-      x = *reinterpret_cast<const uint4*>(static_cast<const T*>(half ? a.values : a.keys) + at + lane * 8);
-    }
-    void* pages = half ? c.values : c.keys;
-    const int64_t to = slot.at + head * c.head_stride + lane * 8;
+    if (item.live) slot = slots[item.t];
+    void* pages = item.half ? c.values : c.keys;
+    const int64_t to = slot.at + item.head * c.head_stride + item.lane * 8;
     if constexpr (!Q8) {
-      if (slot.at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(pages) + to) = x;
+      if (slot.at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(pages) + to) = x[i];
     } else {
-      const float2 f0 = Pair<T>::unpack(x.x), f1 = Pair<T>::unpack(x.y), f2 = Pair<T>::unpack(x.z), f3 = Pair<T>::unpack(x.w);
+      const float2 f0 = Pair<T>::unpack(x[i].x), f1 = Pair<T>::unpack(x[i].y), f2 = Pair<T>::unpack(x[i].z), f3 = Pair<T>::unpack(x[i].w);
       uint32_t top = max(max(max(magnitude_bits(f0.x), magnitude_bits(f0.y)), max(magnitude_bits(f1.x), magnitude_bits(f1.y))),
                          max(max(magnitude_bits(f2.x), magnitude_bits(f2.y)), max(magnitude_bits(f3.x), magnitude_bits(f3.y))));
+      // (all lanes, live or not: the shuffles are warp-wide)
       for (int d = lanes >> 1; d >= 1; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
       float scale, inverse;
       e4m3_scale(top, scale, inverse);
@@ -111,22 +142,23 @@ __global__ void __launch_bounds__(NT) append_kernel(SonicCacheAppendArgs a, int 
         const uint2 codes = make_uint2(e4m3_pack4(f0.x * inverse, f0.y * inverse, f1.x * inverse, f1.y * inverse),
                                        e4m3_pack4(f2.x * inverse, f2.y * inverse, f3.x * inverse, f3.y * inverse));
         *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pages) + to) = codes;
-        if (lane == 0) (half ? c.value_scales : c.key_scales)[slot.scale + head * c.scale_head_stride] = scale;
+        if (item.lane == 0) (item.half ? c.value_scales : c.key_scales)[slot.scale + item.head * c.scale_head_stride] = scale;
       }
     }
   }
 }
 
-// Each thread moves 16 cached bytes: 8 values of a 16-bit cache, or 16 codes into 32 bytes.
+// Each thread moves 16 cached bytes an item: 8 values of a 16-bit cache, or 16 codes into 32 bytes;
+// all items' loads at once.
 template <typename T, bool Q8>
-__global__ void __launch_bounds__(NT) gather_kernel(SonicCacheGatherArgs a, int run, int row_shift) {
+__global__ void __launch_bounds__(NT) gather_kernel(SonicCacheGatherArgs a, Work work) {
   __shared__ Slot slots[MAX_RUN];
   grid_dependency_trigger();
-  grid_dependency_wait();
   const SonicSequences& s = a.sequences;
   const SonicPagedCache& c = a.cache;
-  const int first = blockIdx.x * run;
-  const int count = min(run, s.tokens - first);
+  const int first = blockIdx.x * work.run;
+  const int count = min(work.run, s.tokens - first);
+  grid_dependency_wait();
   if (threadIdx.x < count) {
     const int row = first + threadIdx.x;
     const int b = request_of(a.starts, s.requests, row);
@@ -135,42 +167,47 @@ __global__ void __launch_bounds__(NT) gather_kernel(SonicCacheGatherArgs a, int 
     slots[threadIdx.x] = found;
   }
   __syncthreads();
-  constexpr int PER = Q8 ? 16 : 8;  // values a thread
-  const int lanes = 1 << row_shift;
-  const int lane = threadIdx.x & (lanes - 1);
-  const int rows = count * c.kv_heads * 2;
-  for (int r = threadIdx.x >> row_shift; r < rows; r += NT >> row_shift) {
-    // heads innermost: the rows of a token are neighbours in the output
-    const int head = r % c.kv_heads, half = (r / c.kv_heads) & 1, t = r / (2 * c.kv_heads);
-    const Slot slot = slots[t];
-    uint4 x = make_uint4(0, 0, 0, 0);
-    float scale = 0.0f;
-    if (slot.at >= 0) {
-      const int64_t at = slot.at + head * c.head_stride + lane * PER;
-      const void* pages = half ? c.values : c.keys;
-      if constexpr (Q8) {
-        x = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pages) + at);
-        scale = (half ? c.value_scales : c.key_scales)[slot.scale + head * c.scale_head_stride];
-      } else {
-        x = *reinterpret_cast<const uint4*>(static_cast<const T*>(pages) + at);
-      }
-    }
-    T* out = static_cast<T*>(half ? a.values : a.keys) +
-             ((int64_t)(first + t) * c.kv_heads + head) * c.head_dim + lane * PER;
-    if constexpr (!Q8) {
-      *reinterpret_cast<uint4*>(out) = x;
+  constexpr int PER = Q8 ? 16 : 8;  // values an item
+  uint4 x[ITEMS];
+  float scale[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const Item item = item_of(work, i, count, c.kv_heads);
+    x[i] = make_uint4(0, 0, 0, 0);
+    scale[i] = 0.0f;
+    if (!item.live) continue;
+    const Slot slot = slots[item.t];
+    if (slot.at < 0) continue;
+    const int64_t at = slot.at + item.head * c.head_stride + item.lane * PER;
+    const void* pages = item.half ? c.values : c.keys;
+    if constexpr (Q8) {
+      x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pages) + at);
+      scale[i] = (item.half ? c.value_scales : c.key_scales)[slot.scale + item.head * c.scale_head_stride];
     } else {
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+      x[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(pages) + at);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const Item item = item_of(work, i, count, c.kv_heads);
+    if (!item.live) continue;
+    // (streaming stores: nothing here is read again)
+    T* out = static_cast<T*>(item.half ? a.values : a.keys) +
+             ((int64_t)(first + item.t) * c.kv_heads + item.head) * c.head_dim + item.lane * PER;
+    if constexpr (!Q8) {
+      __stcs(reinterpret_cast<uint4*>(out), x[i]);
+    } else {
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
       uint32_t y[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 lo = Pair<__half>::unpack(e4m3_to_half2((uint16_t)w[i]));
-        const float2 hi = Pair<__half>::unpack(e4m3_to_half2((uint16_t)(w[i] >> 16)));
-        y[2 * i] = Pair<T>::pack(lo.x * scale, lo.y * scale);
-        y[2 * i + 1] = Pair<T>::pack(hi.x * scale, hi.y * scale);
+      for (int k = 0; k < 4; ++k) {
+        const float2 lo = Pair<__half>::unpack(e4m3_to_half2((uint16_t)w[k]));
+        const float2 hi = Pair<__half>::unpack(e4m3_to_half2((uint16_t)(w[k] >> 16)));
+        y[2 * k] = Pair<T>::pack(lo.x * scale[i], lo.y * scale[i]);
+        y[2 * k + 1] = Pair<T>::pack(hi.x * scale[i], hi.y * scale[i]);
       }
-      reinterpret_cast<uint4*>(out)[0] = make_uint4(y[0], y[1], y[2], y[3]);
-      reinterpret_cast<uint4*>(out)[1] = make_uint4(y[4], y[5], y[6], y[7]);
+      __stcs(reinterpret_cast<uint4*>(out), make_uint4(y[0], y[1], y[2], y[3]));
+      __stcs(reinterpret_cast<uint4*>(out) + 1, make_uint4(y[4], y[5], y[6], y[7]));
     }
   }
 }
@@ -181,12 +218,22 @@ int log2_of(int v) {
   return l;
 }
 
-// Tokens a CTA takes: enough that a thread moves several pieces, few enough that a small call
-// still covers the SMs.
-int run_of(int tokens, int pieces_per_token) {
-  const int full = std::max(1, 4 * NT / pieces_per_token);
-  const int spread = std::max(1, tokens / 296);
-  return std::min(MAX_RUN, std::min(full, spread));
+// As many tokens a CTA as its threads take with ITEMS pieces each (one at least, in several rounds of
+// CTAs where a token has more); a small call's are spread over more CTAs.
+Work work_of(int tokens, int heads, int lanes) {
+  Work w;
+  w.row_shift = log2_of(lanes);
+  w.per_token = 2 * heads;
+  w.inverse = (uint32_t)((1ull << 32) / w.per_token + 1);
+  const int full = ITEMS * NT / (2 * heads * lanes), spread = std::max(1, tokens / 296);
+  w.run = std::max(1, std::min(MAX_RUN, std::min(full, spread)));
+  return w;
+}
+
+// blockIdx.y: rounds of a token with more pieces than one CTA takes
+dim3 grid_of(const Work& w, int tokens, int lanes) {
+  const int pieces = w.run * w.per_token * lanes;
+  return dim3((tokens + w.run - 1) / w.run, (pieces + ITEMS * NT - 1) / (ITEMS * NT));
 }
 
 bool is_16bit(int dtype) { return dtype == SONIC_DTYPE_BF16 || dtype == SONIC_DTYPE_F16; }
@@ -238,11 +285,11 @@ extern "C" sonic_status sonic_cache_append(const SonicCacheAppendArgs* a, void* 
       a->value_token_stride % 8 || a->value_head_stride % 8)
     return fail_with(SONIC_ERR_INVALID_ARGUMENT, "rows of keys and values must start on 16-byte boundaries");
   const int lanes = a->cache.head_dim / 8;
-  const int run = run_of(a->sequences.tokens, 2 * a->cache.kv_heads * lanes);
-  const dim3 grid((a->sequences.tokens + run - 1) / run);
+  const Work work = work_of(a->sequences.tokens, a->cache.kv_heads, lanes);
+  const dim3 grid = grid_of(work, a->sequences.tokens, lanes);
   const bool pdl = a->flags & SONIC_FLAG_PDL;
   const auto go = [&](auto kernel) {
-    return launch_status(launch_kernel(kernel, grid, dim3(NT), 0, (cudaStream_t)stream, pdl, 1, *a, run, log2_of(lanes)));
+    return launch_status(launch_kernel(kernel, grid, dim3(NT), 0, (cudaStream_t)stream, pdl, 1, *a, work));
   };
   const bool q8 = a->cache.dtype == SONIC_DTYPE_E4M3;
   if (a->dtype == SONIC_DTYPE_BF16) return q8 ? go(append_kernel<__nv_bfloat16, true>) : go(append_kernel<__nv_bfloat16, false>);
@@ -261,11 +308,11 @@ extern "C" sonic_status sonic_cache_gather(const SonicCacheGatherArgs* a, void* 
     return fail_with(SONIC_ERR_INVALID_ARGUMENT, "outputs must start on 16-byte boundaries");
   const bool q8 = a->cache.dtype == SONIC_DTYPE_E4M3;
   const int lanes = a->cache.head_dim / (q8 ? 16 : 8);
-  const int run = run_of(a->sequences.tokens, 2 * a->cache.kv_heads * lanes);
-  const dim3 grid((a->sequences.tokens + run - 1) / run);
+  const Work work = work_of(a->sequences.tokens, a->cache.kv_heads, lanes);
+  const dim3 grid = grid_of(work, a->sequences.tokens, lanes);
   const bool pdl = a->flags & SONIC_FLAG_PDL;
   const auto go = [&](auto kernel) {
-    return launch_status(launch_kernel(kernel, grid, dim3(NT), 0, (cudaStream_t)stream, pdl, 1, *a, run, log2_of(lanes)));
+    return launch_status(launch_kernel(kernel, grid, dim3(NT), 0, (cudaStream_t)stream, pdl, 1, *a, work));
   };
   if (a->dtype == SONIC_DTYPE_BF16) return q8 ? go(gather_kernel<__nv_bfloat16, true>) : go(gather_kernel<__nv_bfloat16, false>);
   return q8 ? go(gather_kernel<__half, true>) : go(gather_kernel<__half, false>);

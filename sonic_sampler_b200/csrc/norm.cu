@@ -76,12 +76,19 @@ __device__ __forceinline__ float row_sum(float v, int warps, float* shared) {
   return v;
 }
 
-__device__ __forceinline__ uint32_t row_max(uint32_t v, int warps, uint32_t* shared) {
-  v = __reduce_max_sync(0xffffffffu, v);
-  if (warps == 1) return v;
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
+// Both at once, behind one barrier.
+__device__ __forceinline__ void row_sum_and_max(float& v, uint32_t& top, int warps, float* sums, uint32_t* tops) {
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (warps == 1) return;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) sums[threadIdx.x >> 5] = v, tops[threadIdx.x >> 5] = top;
   __syncthreads();
-  return __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < warps ? shared[threadIdx.x & 31] : 0u);
+  v = lane < warps ? sums[lane] : 0.0f;
+  top = __reduce_max_sync(0xffffffffu, lane < warps ? tops[lane] : 0u);
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
 }
 
 // N: items a lane; VEC: 16-byte pieces. blockDim.x = 32 * warps of a row, blockDim.y = rows a CTA
@@ -157,9 +164,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
       }
     }
   }
-  const float rstd = __frsqrt_rn(__fdiv_rn(row_sum(sum, warps, sums), (float)a.hidden) + a.eps);
-
-  uint32_t top = 0;
+  // z = r * weight; y = z * rstd
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if constexpr (VEC) {
@@ -168,18 +173,20 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
       if (column(i, 0) < a.hidden) ws = __ldg(reinterpret_cast<const uint4*>(weight + column(i, 0)));
       Piece<T>::unpack(ws, w);
 #pragma unroll
-      for (int j = 0; j < P; ++j) r[i][j] = column(i, 0) < a.hidden ? r[i][j] * rstd * w[j] : 0.0f;
+      for (int j = 0; j < P; ++j) r[i][j] = column(i, 0) < a.hidden ? r[i][j] * w[j] : 0.0f;
     } else {
 #pragma unroll
-      for (int j = 0; j < P; ++j)
-        r[i][j] = column(i, j) < a.hidden ? r[i][j] * rstd * to_float(weight[column(i, j)]) : 0.0f;
+      for (int j = 0; j < P; ++j) r[i][j] = column(i, j) < a.hidden ? r[i][j] * to_float(weight[column(i, j)]) : 0.0f;
     }
   }
 
   if constexpr (!Q8) {
+    const float rstd = __frsqrt_rn(__fdiv_rn(row_sum(sum, warps, sums), (float)a.hidden) + a.eps);
     T* out = static_cast<T*>(a.out) + row * a.out_stride;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
+#pragma unroll
+      for (int j = 0; j < P; ++j) r[i][j] *= rstd;
       if constexpr (VEC) {
         if (column(i, 0) < a.hidden) *reinterpret_cast<uint4*>(out + column(i, 0)) = Piece<T>::pack(r[i]);
       } else {
@@ -189,15 +196,34 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
       }
     }
   } else {
+    // The codes of a row or group do not depend on rstd, which its largest |y| shares: they are
+    // e4m3(z * (448 / max |z|)), one rounding less on the way. Only a row whose largest |y| lies below
+    // the scales' floor is mapped by rstd * 448 / floor.
     uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.out_stride;
-    float scale, inverse;
+    float rstd, scale, factor;
+    const auto scale_of = [&](uint32_t top) {
+      const float z = __uint_as_float(top), c = z * rstd;
+      if (c < kScaleFloor) {
+        scale = kScaleFloor / kE4m3Max;
+        factor = rstd * (kE4m3Max / kScaleFloor);
+      } else {
+        scale = __fdiv_rn(c, kE4m3Max);
+        // (448 / z would overflow for the tiniest z); a NaN makes the whole row NaN
+        factor = !(c == c) ? c : z < kScaleFloor ? rstd * __fdiv_rn(kE4m3Max, c) : __fdiv_rn(kE4m3Max, z);
+      }
+    };
     if (a.group == 0) {
+      uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int j = 0; j < P; ++j) top = max(top, magnitude_bits(r[i][j]));
-      e4m3_scale(row_max(top, warps, tops), scale, inverse);
+      row_sum_and_max(sum, top, warps, sums, tops);
+      rstd = __frsqrt_rn(__fdiv_rn(sum, (float)a.hidden) + a.eps);
+      scale_of(top);
       if (threadIdx.x == 0) a.scales[row] = scale;
+    } else {
+      rstd = __frsqrt_rn(__fdiv_rn(row_sum(sum, warps, sums), (float)a.hidden) + a.eps);
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -209,15 +235,15 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
         for (int j = 0; j < P; ++j) t = max(t, magnitude_bits(r[i][j]));
 #pragma unroll
         for (int d = LANES / 2; d >= 1; d >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, d));
-        e4m3_scale(t, scale, inverse);
+        scale_of(t);
         const int at = VEC ? column(i, 0) : (i * warps + warp) * 128;
         if (at < a.hidden && lane % LANES == 0) a.scales[row * ((a.hidden + 127) / 128) + at / 128] = scale;
       }
       if constexpr (VEC) {
         if (column(i, 0) < a.hidden) {
-          const uint32_t lo = e4m3_pack4(r[i][0] * inverse, r[i][1] * inverse, r[i][2] * inverse, r[i][3] * inverse);
+          const uint32_t lo = e4m3_pack4(r[i][0] * factor, r[i][1] * factor, r[i][2] * factor, r[i][3] * factor);
           if constexpr (P == 8) {
-            const uint32_t hi = e4m3_pack4(r[i][4] * inverse, r[i][5] * inverse, r[i][6] * inverse, r[i][7] * inverse);
+            const uint32_t hi = e4m3_pack4(r[i][4] * factor, r[i][5] * factor, r[i][6] * factor, r[i][7] * factor);
             *reinterpret_cast<uint2*>(out + column(i, 0)) = make_uint2(lo, hi);
           } else {
             *reinterpret_cast<uint32_t*>(out + column(i, 0)) = lo;
@@ -226,7 +252,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
       } else {
 #pragma unroll
         for (int j = 0; j < P; ++j)
-          if (column(i, j) < a.hidden) out[column(i, j)] = (uint8_t)e4m3_pack2(r[i][j] * inverse, 0.0f);
+          if (column(i, j) < a.hidden) out[column(i, j)] = (uint8_t)e4m3_pack2(r[i][j] * factor, 0.0f);
       }
     }
   }

@@ -7,7 +7,6 @@ side of a speculative verification (`UnshardedFusedMultistep` then judges its lo
 
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 
 import torch
@@ -28,6 +27,9 @@ class PagedAttention:
     pdl: bool
     # zero-filled workspace of the kernel; calls that overlap on the GPU need objects of their own
     scratchpad: Tensor
+
+    def __post_init__(self):
+        self.template = ops.paged_attention_template(self.q_heads, self.head_dim, FLAG_PDL if self.pdl else 0)
 
     @classmethod
     def initialize(cls, q_heads: int, kv_heads: int, head_dim: int, lookahead: int = 0, pdl: bool = True) -> "PagedAttention":
@@ -61,23 +63,18 @@ class PagedAttention:
         `[tokens, q_heads]` logarithms of the softmax sums, with which outputs over disjoint key
         ranges can be joined. A query that sees no key gives zeros and -infinity."""
         ops._require_cuda(queries)
-        shape, struct, device = queries.shape, cache.struct, cache.device
-        if len(shape) != 3 or shape[1] != self.q_heads or shape[2] != self.head_dim:
-            raise ValueError(f"`queries` must be [tokens, {self.q_heads}, {self.head_dim}], got {list(shape)}")
+        struct, device, scratchpad = cache.struct, cache.device, self.scratchpad
         if struct.kv_heads != self.kv_heads or struct.head_dim != self.head_dim:
             raise ValueError("the cache's kv_heads and head_dim must match `initialize`'s")
         if window is None:
             window = 0
         elif window < 1:
             raise ValueError(f"`window` must be positive, got {window}")
-        if self.scratchpad.device != device:
-            raise ValueError(f"the cache is on {device}, this object's workspace on {self.scratchpad.device}")
-        out = queries.new_empty(shape) if output is None else output
-        lse = queries.new_empty(shape[:2], dtype=torch.float32) if logsumexp else None
-        args = ops.paged_attention_args(
-            struct, queries, page_table, lengths, out, cu_seqlens=cu_seqlens,
-            max_tokens=self.lookahead + 1 if cu_seqlens is not None else 0, window=window,
-            scale=1.0 / math.sqrt(self.head_dim) if scale is None else scale, lse=lse, flags=FLAG_PDL if self.pdl else 0,
-            workspace=self.scratchpad, device=device)
+        if scratchpad.device != device:
+            raise ValueError(f"the cache is on {device}, this object's workspace on {scratchpad.device}")
+        args, out, lse = ops.paged_attention_args(
+            self.template, struct, queries, page_table, lengths, cu_seqlens=cu_seqlens,
+            max_tokens=self.lookahead + 1 if cu_seqlens is not None else 0, window=window, scale=scale, out=output,
+            logsumexp=logsumexp, workspace=scratchpad, device=device)
         ops.launch_paged_attention(args, device)
         return (out, lse) if logsumexp else out

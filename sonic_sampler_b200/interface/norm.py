@@ -37,6 +37,7 @@ class ResidualNorm:
             raise ValueError(f"`group` must be 128 (with a float8_e4m3fn output) or None, got {self.group}")
         if not self.eps >= 0.0:
             raise ValueError(f"`eps` must not be negative, got {self.eps}")
+        self.template = ops.residual_norm_template(self.weight, self.dtype, self.eps, self.group or 0, FLAG_PDL if self.pdl else 0)
 
     def __call__(self, x: Tensor, residual: Tensor | None = None, residual_out: Tensor | None = None, out: Tensor | None = None,
                  scales: Tensor | None = None) -> tuple[Tensor, Tensor | None, Tensor | None]:
@@ -46,20 +47,13 @@ class ResidualNorm:
         r, rounded to the input's dtype, is None without a `residual`. `out`, `scales` and
         `residual_out` may give the tensors to write; `residual_out` may be `residual` or `x`."""
         ops._require_cuda(x)
-        shape, hidden = x.shape, self.weight.shape[0]
-        if not shape or shape[-1] != hidden:
-            raise ValueError(f"`x` must have {hidden} columns, got {list(shape)}")
-        if out is None:
-            out = x.new_empty(shape, dtype=self.dtype)
-        if scales is None and out.dtype == E4M3:
-            groups = -(-hidden // self.group) if self.group else 1
-            scales = x.new_empty((*shape[:-1], groups), dtype=torch.float32)
-        if residual is not None and residual_out is None:
-            residual_out = x.new_empty(shape)
-        flat = (x, out, residual, residual_out, scales)
-        if len(shape) != 2:
-            flat = [t if t is None else t.view(-1, t.size(-1)) for t in flat]
-        args = ops.residual_norm_args(flat[0], self.weight, flat[1], residual=flat[2], residual_out=flat[3], scales=flat[4],
-                                      eps=self.eps, group=self.group or 0, flags=FLAG_PDL if self.pdl else 0)
+        if x.dim() != 2:
+            def rows(t):
+                return t if t is None else t.view(-1, t.size(-1))
+
+            y, scales, r = self(rows(x), rows(residual), rows(residual_out), rows(out), rows(scales))
+            lead = x.shape[:-1]
+            return tuple(t if t is None else t.view(*lead, t.size(-1)) for t in (y, scales, r))
+        args, out, scales, residual_out = ops.residual_norm_args(self.template, x, self.weight, residual, residual_out, out, scales)
         ops.launch_residual_norm(args, x.device)
         return out, scales, residual_out

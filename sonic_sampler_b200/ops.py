@@ -10,6 +10,7 @@ tensors' device. Dtype / layout contracts follow the reference's SamplingBuffers
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 from torch import Tensor
@@ -479,30 +480,23 @@ def paged_cache_struct(keys: Tensor, values: Tensor, key_scales: Tensor | None, 
     return c
 
 
-# The builders below run once a call of a decode step: messages are formatted only where a check
-# fails, and each attribute of a tensor is asked for once.
+# The builders below run once a call of a decode step, where the host's time shows: messages are
+# formatted only where a check fails, each attribute of a tensor is asked for once, the fields that
+# an interface object never changes come from its template, and outputs that are allocated here
+# need no checks.
 
 
-def _index_vector(t: Tensor, name: str, size: int, device: torch.device) -> int:
-    if t.dtype != I32 or t.shape != (size,) or (size > 1 and t.stride(0) != 1):
-        raise ValueError(f"`{name}` must be a contiguous int32 vector of {size} entries")
-    if t.device != device:
-        raise ValueError(f"`{name}` must be on {device}")
-    return t.data_ptr()
-
-
-def _sequences(s: SequencesStruct, tokens: int, page_table: Tensor, lengths: Tensor | None, cu_seqlens: Tensor | None,
-               device: torch.device) -> int:
-    """Fill `s`; returns the number of requests."""
-    shape = page_table.shape
-    if page_table.dtype != I32 or len(shape) != 2:
+def _sequences(a, tokens: int, page_table: Tensor, lengths: Tensor | None, cu_seqlens: Tensor | None, device: torch.device) -> int:
+    """Fill `a.sequences`; returns the number of requests."""
+    if page_table.dtype != I32 or page_table.dim() != 2:
         raise ValueError("`page_table` must be int32 [requests, pages] with a unit inner stride")
-    requests, width = shape
+    requests, width = page_table.shape
     row, inner = page_table.stride()
     if inner != 1 and width > 1:
         raise ValueError("`page_table` must be int32 [requests, pages] with a unit inner stride")
     if page_table.device != device:
         raise ValueError(f"`page_table` must be on {device}")
+    s = a.sequences
     s.requests = requests
     s.table_width = width
     s.table_stride = row
@@ -517,14 +511,24 @@ def _sequences(s: SequencesStruct, tokens: int, page_table: Tensor, lengths: Ten
     return requests
 
 
-def _token_rows(t: Tensor, name: str, heads: int, head_dim: int, device: torch.device) -> tuple[int, int, int]:
-    """(tokens, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim or stride[2] != 1:
-        raise ValueError(f"`{name}` must be [tokens, {heads}, {head_dim}] with a unit inner stride")
+def _index_vector(t: Tensor, name: str, size: int, device: torch.device) -> int:
+    if t.dtype != I32 or t.dim() != 1 or t.size(0) != size or (size > 1 and t.stride(0) != 1):
+        raise ValueError(f"`{name}` must be a contiguous int32 vector of {size} entries")
     if t.device != device:
         raise ValueError(f"`{name}` must be on {device}")
-    return shape[0], stride[0], stride[1]
+    return t.data_ptr()
+
+
+def _token_rows(t: Tensor, name: str, heads: int, head_dim: int, device: torch.device) -> tuple[int, int, int]:
+    """(tokens, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
+    if t.dim() == 3:
+        tokens, h, d = t.shape
+        token_stride, head_stride, inner = t.stride()
+        if h == heads and d == head_dim and inner == 1:
+            if t.device != device:
+                raise ValueError(f"`{name}` must be on {device}")
+            return tokens, token_stride, head_stride
+    raise ValueError(f"`{name}` must be [tokens, {heads}, {head_dim}] with a unit inner stride")
 
 
 def cache_append_args(cache: PagedCacheStruct, keys: Tensor, values: Tensor, page_table: Tensor, lengths: Tensor, *,
@@ -538,7 +542,7 @@ def cache_append_args(cache: PagedCacheStruct, keys: Tensor, values: Tensor, pag
     dtype = keys.dtype
     if dtype not in _ACTIVATION_DTYPES or values.dtype != dtype:
         raise ValueError("`keys` and `values` must both be bf16 or fp16")
-    _sequences(a.sequences, tokens, page_table, lengths, cu_seqlens, device)
+    _sequences(a, tokens, page_table, lengths, cu_seqlens, device)
     a.cache = cache
     a.flags = flags
     a.dtype = _ACTIVATION_DTYPES[dtype]
@@ -549,18 +553,24 @@ def cache_append_args(cache: PagedCacheStruct, keys: Tensor, values: Tensor, pag
     return a
 
 
-def cache_gather_args(cache: PagedCacheStruct, page_table: Tensor, starts: Tensor, keys: Tensor, values: Tensor, *,
-                      flags: int, error: Tensor | None, device: torch.device) -> CacheGatherArgs:
+def cache_gather_args(cache: PagedCacheStruct, page_table: Tensor, starts: Tensor, total: int, dtype: torch.dtype,
+                      keys: Tensor | None, values: Tensor | None, *, flags: int, error: Tensor | None,
+                      device: torch.device) -> tuple[CacheGatherArgs, Tensor, Tensor]:
+    """The arguments, and the outputs (allocated where they are None)."""
     a = CacheGatherArgs()
     heads, dim = cache.kv_heads, cache.head_dim
-    tokens, _, _ = _token_rows(keys, "keys", heads, dim, device)
-    rows, _, _ = _token_rows(values, "values", heads, dim, device)
-    if rows != tokens:
-        raise ValueError("`keys` and `values` must have the same number of rows")
-    dtype = keys.dtype
-    if dtype not in _ACTIVATION_DTYPES or values.dtype != dtype or not keys.is_contiguous() or not values.is_contiguous():
-        raise ValueError("`keys` and `values` must both be contiguous and bf16 or fp16")
-    requests = _sequences(a.sequences, tokens, page_table, None, None, device)
+    if dtype not in _ACTIVATION_DTYPES:
+        raise ValueError("`keys` and `values` must be bf16 or fp16")
+    shape, strides = (total, heads, dim), (heads * dim, dim, 1)
+    if keys is None:
+        keys = torch.empty_strided(shape, strides, dtype=dtype, device=device)
+    elif _token_rows(keys, "keys", heads, dim, device)[0] != total or keys.dtype != dtype or not keys.is_contiguous():
+        raise ValueError(f"`keys` must be contiguous {dtype} of {total} rows")
+    if values is None:
+        values = torch.empty_strided(shape, strides, dtype=dtype, device=device)
+    elif _token_rows(values, "values", heads, dim, device)[0] != total or values.dtype != dtype or not values.is_contiguous():
+        raise ValueError(f"`values` must be contiguous {dtype} of {total} rows")
+    requests = _sequences(a, total, page_table, None, None, device)
     a.starts = _index_vector(starts, "starts", requests + 1, device)
     a.cache = cache
     a.flags = flags
@@ -569,40 +579,64 @@ def cache_gather_args(cache: PagedCacheStruct, page_table: Tensor, starts: Tenso
     a.values = values.data_ptr()
     a.error = _ptr(error)
     a._tensors = (cache, page_table, starts, keys, values, error)
+    return a, keys, values
+
+
+def paged_attention_template(q_heads: int, head_dim: int, flags: int) -> PagedAttentionArgs:
+    a = PagedAttentionArgs()
+    a.q_heads = q_heads
+    a.flags = flags
+    a.scale = 1.0 / math.sqrt(head_dim)
     return a
 
 
-def paged_attention_args(cache: PagedCacheStruct, queries: Tensor, page_table: Tensor, lengths: Tensor, out: Tensor, *,
-                         cu_seqlens: Tensor | None, max_tokens: int, window: int, scale: float, lse: Tensor | None, flags: int,
-                         workspace: Tensor | None, device: torch.device) -> PagedAttentionArgs:
-    a = PagedAttentionArgs()
-    dim = cache.head_dim
-    heads = queries.shape[1] if queries.dim() == 3 else -1
+def paged_attention_args(template: PagedAttentionArgs, cache: PagedCacheStruct, queries: Tensor, page_table: Tensor,
+                         lengths: Tensor, *, cu_seqlens: Tensor | None, max_tokens: int, window: int, scale: float | None,
+                         out: Tensor | None, logsumexp: bool, workspace: Tensor, device: torch.device
+                         ) -> tuple[PagedAttentionArgs, Tensor, Tensor | None]:
+    """The arguments, the output (allocated where `out` is None) and the log-sum-exps, if asked for."""
+    a = PagedAttentionArgs.from_buffer_copy(template)
+    heads, dim = a.q_heads, cache.head_dim
     tokens, a.q_token_stride, a.q_head_stride = _token_rows(queries, "queries", heads, dim, device)
-    rows, a.out_token_stride, a.out_head_stride = _token_rows(out, "output", heads, dim, device)
     dtype = queries.dtype
-    if rows != tokens or out.dtype != dtype:
-        raise ValueError("`output` must match `queries` in shape and dtype")
     if dtype not in _ACTIVATION_DTYPES:
         raise ValueError("`queries` must be bf16 or fp16")
-    _sequences(a.sequences, tokens, page_table, lengths, cu_seqlens, device)
+    if out is None:
+        out = torch.empty_strided((tokens, heads, dim), (heads * dim, dim, 1), dtype=dtype, device=device)
+        a.out_token_stride = heads * dim
+        a.out_head_stride = dim
+    else:
+        rows, a.out_token_stride, a.out_head_stride = _token_rows(out, "output", heads, dim, device)
+        if rows != tokens or out.dtype != dtype:
+            raise ValueError("`output` must match `queries` in shape and dtype")
+    lse = None
+    if logsumexp:
+        lse = torch.empty_strided((tokens, heads), (heads, 1), dtype=F32, device=device)
+        a.lse = lse.data_ptr()
+    _sequences(a, tokens, page_table, lengths, cu_seqlens, device)
     a.cache = cache
-    a.flags = flags
     a.dtype = _ACTIVATION_DTYPES[dtype]
-    a.q_heads = heads
     a.max_tokens = max_tokens
     a.window = window
-    a.scale = scale
+    if scale is not None:
+        a.scale = scale
     a.queries = queries.data_ptr()
     a.out = out.data_ptr()
-    if lse is not None:
-        if lse.dtype != F32 or lse.shape != (tokens, heads) or not lse.is_contiguous() or lse.device != device:
-            raise ValueError("`logsumexp` must be a contiguous fp32 [tokens, q_heads] tensor on the queries' device")
-        a.lse = lse.data_ptr()
-    if workspace is not None:
-        a.workspace = workspace.data_ptr()
-        a.workspace_bytes = workspace.nbytes
+    a.workspace = workspace.data_ptr()
+    a.workspace_bytes = workspace.numel()
     a._tensors = (cache, queries, page_table, lengths, cu_seqlens, out, lse, workspace)
+    return a, out, lse
+
+
+def residual_norm_template(weight: Tensor, out_dtype: torch.dtype | None, eps: float, group: int, flags: int) -> ResidualNormArgs:
+    _require(weight.dim() == 1 and weight.dtype in _NORM_DTYPES and (weight.size(0) <= 1 or weight.stride(0) == 1),
+             "`weight` must be a contiguous bf16, fp16 or fp32 vector")
+    a = ResidualNormArgs()
+    a.hidden = weight.size(0)
+    a.dtype = a.out_dtype = _NORM_DTYPES[weight.dtype]
+    if out_dtype == E4M3:
+        a.out_dtype = DT_E4M3
+    a.group, a.eps, a.flags = group, eps, flags
     return a
 
 
@@ -616,43 +650,48 @@ def _norm_rows(t: Tensor, name: str, rows: int, hidden: int, dtype: torch.dtype,
     return row
 
 
-def residual_norm_args(x: Tensor, weight: Tensor, out: Tensor, *, residual: Tensor | None, residual_out: Tensor | None,
-                       scales: Tensor | None, eps: float, group: int, flags: int) -> ResidualNormArgs:
-    a = ResidualNormArgs()
-    dtype, device = x.dtype, x.device
-    if x.dim() != 2 or dtype not in _NORM_DTYPES:
-        raise ValueError("`x` must be a bf16, fp16 or fp32 [rows, hidden] tensor")
-    rows, hidden = x.shape
+def residual_norm_args(template: ResidualNormArgs, x: Tensor, weight: Tensor, residual: Tensor | None, residual_out: Tensor | None,
+                       out: Tensor | None, scales: Tensor | None) -> tuple[ResidualNormArgs, Tensor, Tensor | None, Tensor | None]:
+    """The arguments, and the outputs (out, scales, residual_out; allocated where they are needed and None)."""
+    a = ResidualNormArgs.from_buffer_copy(template)
+    dtype, device, hidden = weight.dtype, weight.device, a.hidden
+    if x.dim() != 2 or x.size(1) != hidden:
+        raise ValueError(f"`x` must have {hidden} columns, got {list(x.shape)}")
+    if x.dtype != dtype or x.device != device:
+        raise ValueError(f"`x` must have the weight's dtype and device, {dtype} on {device}")
+    rows = x.size(0)
     a.rows = rows
-    a.hidden = hidden
-    a.dtype = a.out_dtype = _NORM_DTYPES[dtype]
-    a.group = group
-    a.flags = flags
-    a.eps = eps
     a.x_stride = _norm_rows(x, "x", rows, hidden, dtype, device)
     a.x = x.data_ptr()
-    if weight.shape != (hidden,) or weight.dtype != dtype or weight.device != device or (hidden > 1 and weight.stride(0) != 1):
-        raise ValueError(f"`weight` must be a contiguous {dtype} vector of {hidden} entries on {device}")
     a.weight = weight.data_ptr()
     if residual is not None:
         a.residual_stride = _norm_rows(residual, "residual", rows, hidden, dtype, device)
         a.residual = residual.data_ptr()
-    if residual_out is not None:
+        if residual_out is None:
+            residual_out = torch.empty_strided((rows, hidden), (hidden, 1), dtype=dtype, device=device)
+            a.residual_out_stride = hidden
+            a.residual_out = residual_out.data_ptr()
+    if residual_out is not None and not a.residual_out:
         a.residual_out_stride = _norm_rows(residual_out, "residual_out", rows, hidden, dtype, device)
         a.residual_out = residual_out.data_ptr()
-    out_dtype = out.dtype
-    if out_dtype != dtype and out_dtype != E4M3:
-        raise ValueError("`out` must have the dtype of `x`, or be float8_e4m3fn")
-    a.out_stride = _norm_rows(out, "out", rows, hidden, out_dtype, device)
+    if out is not None:  # what is given says which output is wanted
+        a.out_dtype = DT_E4M3 if out.dtype == E4M3 else a.dtype
+    q8 = a.out_dtype == DT_E4M3
+    if out is None:
+        out = torch.empty_strided((rows, hidden), (hidden, 1), dtype=E4M3 if q8 else dtype, device=device)
+        a.out_stride = hidden
+    else:
+        a.out_stride = _norm_rows(out, "out", rows, hidden, E4M3 if q8 else dtype, device)
     a.out = out.data_ptr()
-    if out_dtype == E4M3:
-        a.out_dtype = DT_E4M3
-        groups = -(-hidden // group) if group else 1
-        if scales is None or scales.dtype != F32 or scales.shape != (rows, groups) or not scales.is_contiguous() or scales.device != device:
+    if q8:
+        groups = -(-hidden // a.group) if a.group else 1
+        if scales is None:
+            scales = torch.empty_strided((rows, groups), (groups, 1), dtype=F32, device=device)
+        elif scales.dtype != F32 or scales.shape != (rows, groups) or not scales.is_contiguous() or scales.device != device:
             raise ValueError(f"`scales` must be a contiguous fp32 [{rows}, {groups}] tensor on {device}")
         a.scales = scales.data_ptr()
     a._tensors = (x, weight, out, residual, residual_out, scales)
-    return a
+    return a, out, scales, residual_out
 
 
 def paged_attention_workspace_bytes() -> int:
