@@ -14,7 +14,7 @@
 namespace sonic {
 namespace {
 
-constexpr int NT = 256;
+constexpr int NT = 128;  // (256: 4 % slower read-back, 2 % slower append)
 constexpr int MAX_RUN = 64;  // tokens a CTA takes at most
 
 // Request of row `row`: the last b with bounds[b] <= row (bounds non-decreasing, bounds[0] <= row).
@@ -54,8 +54,9 @@ __device__ __forceinline__ Slot find_slot(const SonicPagedCache& c, const SonicS
 }
 
 // Pieces of the run's tokens, `lanes` neighbouring threads a (token, keys or values, head) row: piece
-// i of thread `tid`, of ITEMS a thread at most.
-constexpr int ITEMS = 4;
+// i of a thread, of `items` a thread.
+constexpr int APPEND_ITEMS = 2;
+constexpr int GATHER_ITEMS = 4;
 
 struct Work {
   int run;             // tokens a CTA takes
@@ -69,9 +70,9 @@ struct Item {
   int t, half, head, lane;
 };
 
-__device__ __forceinline__ Item item_of(const Work& w, int i, int count, int heads) {
+__device__ __forceinline__ Item item_of(const Work& w, int i, int count, int heads, int items) {
   Item x;
-  const uint32_t r = ((blockIdx.y * ITEMS + i) * NT + threadIdx.x) >> w.row_shift;
+  const uint32_t r = ((blockIdx.y * items + i) * NT + threadIdx.x) >> w.row_shift;
   x.lane = threadIdx.x & ((1 << w.row_shift) - 1);
   x.live = r < count * w.per_token;
   x.t = __umulhi(r, w.inverse);
@@ -81,10 +82,14 @@ __device__ __forceinline__ Item item_of(const Work& w, int i, int count, int hea
   return x;
 }
 
-// Each thread moves 8 activations an item: 16 bytes in; 16 bytes (16-bit cache) or 8 codes out. A row
-// is head_dim / 8 neighbouring lanes (8, 16 or 32), which reduce its largest magnitude by shuffles.
-// The activations are asked for before the tokens are looked up, all items' at once: 16000 tokens of 8
-// heads of 128 take XXAPPEND us (one item at a time, after the look-up: 34 us).
+// Largest magnitude of a packed pair's lanes and of `top`'s, as 16-bit patterns (NaN above infinity).
+__device__ __forceinline__ uint32_t top_pair(uint32_t top, uint32_t x) { return __vmaxu2(top, x & 0x7fff7fffu); }
+
+// Each thread moves 16 activations an item: 32 bytes in; 32 bytes (16-bit cache) or 16 codes out. A row
+// is head_dim / 16 neighbouring lanes (4, 8 or 16), which reduce its largest magnitude by shuffles, on
+// packed 16-bit patterns. The activations are asked for before the tokens are looked up, all items' at
+// once. Bound by instructions more than by memory: 16000 tokens of 8 heads of 128 into e4m3 take
+// 21 us (8 activations an item, fp32 maxima: 31 us; one item at a time: 34 us).
 template <typename T, bool Q8>
 __global__ void __launch_bounds__(NT) append_kernel(SonicCacheAppendArgs a, Work work) {
   __shared__ Slot slots[MAX_RUN];
@@ -94,15 +99,17 @@ __global__ void __launch_bounds__(NT) append_kernel(SonicCacheAppendArgs a, Work
   const int first = blockIdx.x * work.run;
   const int count = min(work.run, s.tokens - first);
   grid_dependency_wait();
-  uint4 x[ITEMS];
+  uint4 x[APPEND_ITEMS][2];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const Item item = item_of(work, i, count, c.kv_heads);
-    x[i] = make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < APPEND_ITEMS; ++i) {
+    const Item item = item_of(work, i, count, c.kv_heads, APPEND_ITEMS);
+    x[i][0] = x[i][1] = make_uint4(0, 0, 0, 0);
     if (item.live) {
       const int64_t at = item.half ? (first + item.t) * a.value_token_stride + item.head * a.value_head_stride
                                    : (first + item.t) * a.key_token_stride + item.head * a.key_head_stride;
-      x[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(item.half ? a.values : a.keys) + at + item.lane * 8);
+      const uint4* from = reinterpret_cast<const uint4*>(static_cast<const T*>(item.half ? a.values : a.keys) + at + item.lane * 16);
+      x[i][0] = from[0];
+      x[i][1] = from[1];
     }
   }
   if (threadIdx.x < count) {
@@ -122,34 +129,45 @@ __global__ void __launch_bounds__(NT) append_kernel(SonicCacheAppendArgs a, Work
   __syncthreads();
   const int lanes = 1 << work.row_shift;
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const Item item = item_of(work, i, count, c.kv_heads);
+  for (int i = 0; i < APPEND_ITEMS; ++i) {
+    const Item item = item_of(work, i, count, c.kv_heads, APPEND_ITEMS);
     Slot slot;
     if (item.live) slot = slots[item.t];
     void* pages = item.half ? c.values : c.keys;
-    const int64_t to = slot.at + item.head * c.head_stride + item.lane * 8;
+    const int64_t to = slot.at + item.head * c.head_stride + item.lane * 16;
     if constexpr (!Q8) {
-      if (slot.at >= 0) *reinterpret_cast<uint4*>(static_cast<T*>(pages) + to) = x[i];
-    } else {
-      const float2 f0 = Pair<T>::unpack(x[i].x), f1 = Pair<T>::unpack(x[i].y), f2 = Pair<T>::unpack(x[i].z), f3 = Pair<T>::unpack(x[i].w);
-      uint32_t top = max(max(max(magnitude_bits(f0.x), magnitude_bits(f0.y)), max(magnitude_bits(f1.x), magnitude_bits(f1.y))),
-                         max(max(magnitude_bits(f2.x), magnitude_bits(f2.y)), max(magnitude_bits(f3.x), magnitude_bits(f3.y))));
-      // (all lanes, live or not: the shuffles are warp-wide)
-      for (int d = lanes >> 1; d >= 1; d >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-      float scale, inverse;
-      e4m3_scale(top, scale, inverse);
       if (slot.at >= 0) {
-        const uint2 codes = make_uint2(e4m3_pack4(f0.x * inverse, f0.y * inverse, f1.x * inverse, f1.y * inverse),
-                                       e4m3_pack4(f2.x * inverse, f2.y * inverse, f3.x * inverse, f3.y * inverse));
-        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(pages) + to) = codes;
+        reinterpret_cast<uint4*>(static_cast<T*>(pages) + to)[0] = x[i][0];
+        reinterpret_cast<uint4*>(static_cast<T*>(pages) + to)[1] = x[i][1];
+      }
+    } else {
+      const uint32_t w[8] = {x[i][0].x, x[i][0].y, x[i][0].z, x[i][0].w, x[i][1].x, x[i][1].y, x[i][1].z, x[i][1].w};
+      uint32_t top = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) top = top_pair(top, w[k]);
+      // (all lanes, live or not: the shuffles are warp-wide)
+      for (int d = lanes >> 1; d >= 1; d >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
+      top = max(top & 0xffffu, top >> 16);
+      float scale, inverse;
+      e4m3_scale(magnitude_bits(Pair<T>::unpack(top).x), scale, inverse);
+      if (slot.at >= 0) {
+        uint32_t codes[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 lo = Pair<T>::unpack(w[2 * k]), hi = Pair<T>::unpack(w[2 * k + 1]);
+          codes[k] = e4m3_pack4(lo.x * inverse, lo.y * inverse, hi.x * inverse, hi.y * inverse);
+        }
+        *reinterpret_cast<uint4*>(static_cast<uint8_t*>(pages) + to) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
         if (item.lane == 0) (item.half ? c.value_scales : c.key_scales)[slot.scale + item.head * c.scale_head_stride] = scale;
       }
     }
   }
 }
 
-// Each thread moves 16 cached bytes an item: 8 values of a 16-bit cache, or 16 codes into 32 bytes;
-// all items' loads at once.
+// Each thread moves 16 cached bytes an item: 8 values of a 16-bit cache, all items' loads at once, or 16
+// codes into 32 bytes, one item after the other (three bytes move for each one asked for, and
+// more reads in flight only disturb the writes: 215000 tokens of 8 heads of 128 take 206 us, 95 % of the
+// measured copy rate, 241 to 256 us with 2 or 4 items' loads at once; 16-bit: 44 us against 48).
 template <typename T, bool Q8>
 __global__ void __launch_bounds__(NT) gather_kernel(SonicCacheGatherArgs a, Work work) {
   __shared__ Slot slots[MAX_RUN];
@@ -168,46 +186,49 @@ __global__ void __launch_bounds__(NT) gather_kernel(SonicCacheGatherArgs a, Work
   }
   __syncthreads();
   constexpr int PER = Q8 ? 16 : 8;  // values an item
-  uint4 x[ITEMS];
-  float scale[ITEMS];
+  constexpr int AT_ONCE = Q8 ? 1 : GATHER_ITEMS;
+#pragma unroll 1
+  for (int i0 = 0; i0 < GATHER_ITEMS; i0 += AT_ONCE) {
+    uint4 x[AT_ONCE];
+    float scale[AT_ONCE];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const Item item = item_of(work, i, count, c.kv_heads);
-    x[i] = make_uint4(0, 0, 0, 0);
-    scale[i] = 0.0f;
-    if (!item.live) continue;
-    const Slot slot = slots[item.t];
-    if (slot.at < 0) continue;
-    const int64_t at = slot.at + item.head * c.head_stride + item.lane * PER;
-    const void* pages = item.half ? c.values : c.keys;
-    if constexpr (Q8) {
-      x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pages) + at);
-      scale[i] = (item.half ? c.value_scales : c.key_scales)[slot.scale + item.head * c.scale_head_stride];
-    } else {
-      x[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(pages) + at);
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    const Item item = item_of(work, i, count, c.kv_heads);
-    if (!item.live) continue;
-    // (streaming stores: nothing here is read again)
-    T* out = static_cast<T*>(item.half ? a.values : a.keys) +
-             ((int64_t)(first + item.t) * c.kv_heads + item.head) * c.head_dim + item.lane * PER;
-    if constexpr (!Q8) {
-      __stcs(reinterpret_cast<uint4*>(out), x[i]);
-    } else {
-      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      uint32_t y[8];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 lo = Pair<__half>::unpack(e4m3_to_half2((uint16_t)w[k]));
-        const float2 hi = Pair<__half>::unpack(e4m3_to_half2((uint16_t)(w[k] >> 16)));
-        y[2 * k] = Pair<T>::pack(lo.x * scale[i], lo.y * scale[i]);
-        y[2 * k + 1] = Pair<T>::pack(hi.x * scale[i], hi.y * scale[i]);
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const Item item = item_of(work, i0 + i, count, c.kv_heads, GATHER_ITEMS);
+      x[i] = make_uint4(0, 0, 0, 0);
+      scale[i] = 0.0f;
+      if (!item.live) continue;
+      const Slot slot = slots[item.t];
+      if (slot.at < 0) continue;
+      const int64_t at = slot.at + item.head * c.head_stride + item.lane * PER;
+      const void* pages = item.half ? c.values : c.keys;
+      if constexpr (Q8) {
+        x[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(pages) + at);
+        scale[i] = (item.half ? c.value_scales : c.key_scales)[slot.scale + item.head * c.scale_head_stride];
+      } else {
+        x[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(pages) + at);
       }
-      __stcs(reinterpret_cast<uint4*>(out), make_uint4(y[0], y[1], y[2], y[3]));
-      __stcs(reinterpret_cast<uint4*>(out) + 1, make_uint4(y[4], y[5], y[6], y[7]));
+    }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const Item item = item_of(work, i0 + i, count, c.kv_heads, GATHER_ITEMS);
+      if (!item.live) continue;
+      T* out = static_cast<T*>(item.half ? a.values : a.keys) +
+               ((int64_t)(first + item.t) * c.kv_heads + item.head) * c.head_dim + item.lane * PER;
+      if constexpr (!Q8) {
+        *reinterpret_cast<uint4*>(out) = x[i];
+      } else {
+        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+        uint32_t y[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 lo = Pair<__half>::unpack(e4m3_to_half2((uint16_t)w[k]));
+          const float2 hi = Pair<__half>::unpack(e4m3_to_half2((uint16_t)(w[k] >> 16)));
+          y[2 * k] = Pair<T>::pack(lo.x * scale[i], lo.y * scale[i]);
+          y[2 * k + 1] = Pair<T>::pack(hi.x * scale[i], hi.y * scale[i]);
+        }
+        reinterpret_cast<uint4*>(out)[0] = make_uint4(y[0], y[1], y[2], y[3]);
+        reinterpret_cast<uint4*>(out)[1] = make_uint4(y[4], y[5], y[6], y[7]);
+      }
     }
   }
 }
@@ -218,22 +239,22 @@ int log2_of(int v) {
   return l;
 }
 
-// As many tokens a CTA as its threads take with ITEMS pieces each (one at least, in several rounds of
+// As many tokens a CTA as its threads take with APPEND_ITEMS pieces each (one at least, in several rounds of
 // CTAs where a token has more); a small call's are spread over more CTAs.
-Work work_of(int tokens, int heads, int lanes) {
+Work work_of(int tokens, int heads, int lanes, int items) {
   Work w;
   w.row_shift = log2_of(lanes);
   w.per_token = 2 * heads;
   w.inverse = (uint32_t)((1ull << 32) / w.per_token + 1);
-  const int full = ITEMS * NT / (2 * heads * lanes), spread = std::max(1, tokens / 296);
+  const int full = items * NT / (2 * heads * lanes), spread = std::max(1, tokens / 296);
   w.run = std::max(1, std::min(MAX_RUN, std::min(full, spread)));
   return w;
 }
 
 // blockIdx.y: rounds of a token with more pieces than one CTA takes
-dim3 grid_of(const Work& w, int tokens, int lanes) {
+dim3 grid_of(const Work& w, int tokens, int lanes, int items) {
   const int pieces = w.run * w.per_token * lanes;
-  return dim3((tokens + w.run - 1) / w.run, (pieces + ITEMS * NT - 1) / (ITEMS * NT));
+  return dim3((tokens + w.run - 1) / w.run, (pieces + items * NT - 1) / (items * NT));
 }
 
 bool is_16bit(int dtype) { return dtype == SONIC_DTYPE_BF16 || dtype == SONIC_DTYPE_F16; }
@@ -284,9 +305,9 @@ extern "C" sonic_status sonic_cache_append(const SonicCacheAppendArgs* a, void* 
   if (!is_aligned(a->keys, 16) || !is_aligned(a->values, 16) || a->key_token_stride % 8 || a->key_head_stride % 8 ||
       a->value_token_stride % 8 || a->value_head_stride % 8)
     return fail_with(SONIC_ERR_INVALID_ARGUMENT, "rows of keys and values must start on 16-byte boundaries");
-  const int lanes = a->cache.head_dim / 8;
-  const Work work = work_of(a->sequences.tokens, a->cache.kv_heads, lanes);
-  const dim3 grid = grid_of(work, a->sequences.tokens, lanes);
+  const int lanes = a->cache.head_dim / 16;
+  const Work work = work_of(a->sequences.tokens, a->cache.kv_heads, lanes, APPEND_ITEMS);
+  const dim3 grid = grid_of(work, a->sequences.tokens, lanes, APPEND_ITEMS);
   const bool pdl = a->flags & SONIC_FLAG_PDL;
   const auto go = [&](auto kernel) {
     return launch_status(launch_kernel(kernel, grid, dim3(NT), 0, (cudaStream_t)stream, pdl, 1, *a, work));
@@ -308,8 +329,8 @@ extern "C" sonic_status sonic_cache_gather(const SonicCacheGatherArgs* a, void* 
     return fail_with(SONIC_ERR_INVALID_ARGUMENT, "outputs must start on 16-byte boundaries");
   const bool q8 = a->cache.dtype == SONIC_DTYPE_E4M3;
   const int lanes = a->cache.head_dim / (q8 ? 16 : 8);
-  const Work work = work_of(a->sequences.tokens, a->cache.kv_heads, lanes);
-  const dim3 grid = grid_of(work, a->sequences.tokens, lanes);
+  const Work work = work_of(a->sequences.tokens, a->cache.kv_heads, lanes, GATHER_ITEMS);
+  const dim3 grid = grid_of(work, a->sequences.tokens, lanes, GATHER_ITEMS);
   const bool pdl = a->flags & SONIC_FLAG_PDL;
   const auto go = [&](auto kernel) {
     return launch_status(launch_kernel(kernel, grid, dim3(NT), 0, (cudaStream_t)stream, pdl, 1, *a, work));
