@@ -47,9 +47,11 @@ extern "C" sonic_status sonic_paged_attention(const SonicPagedAttentionArgs* a, 
   p.ws.parts = reinterpret_cast<float4*>(w + HEADER + TICKET_BYTES + STAT_BYTES);
   p.group = a->q_heads / a->cache.kv_heads;
   p.group_inverse = (uint32_t)((1ull << 32) / p.group + 1);
-  p.page_shift = -1;
-  for (int i = 0; i < 31; ++i)
-    if (a->cache.page_size == 1 << i) p.page_shift = i;
+  // page_size <= 2^l: the inverse is 2^32 (2^l - page_size) / page_size + 1, the shift l - 1
+  int l = 0;
+  while ((1ll << l) < a->cache.page_size) ++l;
+  p.page_inverse = (uint32_t)(((1ull << 32) * ((1ull << l) - a->cache.page_size)) / a->cache.page_size + 1);
+  p.page_shift = l - 1;
   p.packed = a->cache.slot_stride != a->cache.head_dim || a->cache.page_size % 16 ? 0 : a->cache.page_size % 32 ? 1 : 2;
   const SonicSequences& s = a->sequences;
   p.room = (int)std::min<int64_t>((int64_t)s.table_width * a->cache.page_size, 1 << 30);

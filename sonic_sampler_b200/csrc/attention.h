@@ -34,7 +34,11 @@ struct AttentionLaunch {
   AttentionWorkspace ws;
   int group;               // query heads a kv head
   uint32_t group_inverse;  // floor(2^32 / group) + 1: r / group is the high half of r times it
-  int page_shift;          // log2(page_size), or -1
+  // k / page_size = (h + (k - h) / 2) >> page_shift with h the high half of k times page_inverse
+  // (Granlund and Montgomery, Division by invariant integers using multiplication, 1994); pages of one
+  // slot have the shift -1
+  uint32_t page_inverse;
+  int page_shift;
   int packed;              // a page's rows follow one another, and a page holds a multiple of 16 (1) or 32 (2)
   int room;                // longest request: what a page-table row holds, at most 2^30
   int window;              // 0 where no request is longer than it

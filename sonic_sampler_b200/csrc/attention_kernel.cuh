@@ -294,6 +294,7 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
   __shared__ alignas(16) float2 ring_stats[WARPS][PART_ROWS];
   __shared__ alignas(16) float2 cta_stats[PART_ROWS];  // of a unit's parts in this CTA, joined
   __shared__ uint32_t arrived_last;
+  __shared__ const char* row_address[WARPS][32];  // key rows of a tile that is copied row by row
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;  // fragment row, and pair of columns
   const SonicSequences& seq = p.a.sequences;
@@ -304,6 +305,12 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
   if (tid < 2 * WARPS) shared_live[tid >> 1][tid & 1] = 0;
   grid_dependency_wait();
 
+  // k / page_size, for k below 2^31
+  const auto page_of = [&](int k) {
+    if (p.page_shift < 0) return k;
+    const uint32_t high = __umulhi((uint32_t)k, p.page_inverse);
+    return (int)((high + (((uint32_t)k - high) >> 1)) >> p.page_shift);
+  };
   // query row r of a request belongs to its token r / group
   const auto token_of = [&](int row) { return p.group == 1 ? row : (int)__umulhi((uint32_t)row, p.group_inverse); };
   const auto out_row = [&](const Piece& u, int r) {
@@ -486,7 +493,7 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
           const bool wanted = k + key_span >= from && k < to;
           const bool there = wanted && (uint32_t)pages < (uint32_t)cache.pages;
           if (wanted && !there) atomicOr(p.ws.error, (uint32_t)SONIC_DEVICE_ERR_PAGE);
-          const int slot = p.page_shift >= 0 ? k & (cache.page_size - 1) : k % cache.page_size;
+          const int slot = k - page_of(k) * cache.page_size;
           at = there ? (pages * cache.page_stride + head_at + slot * cache.slot_stride) * (Q8 ? 1 : 2) : 0;
           if constexpr (Q8) scale = there ? pages * cache.scale_page_stride + scale_head_at + slot : 0;
           return there;
@@ -524,18 +531,19 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
             copy16((vd ^ S::value_xor(i)) + i * 512, from16 + value_delta);
           }
         } else {
-          // row by row: lane r's address is that of key r
+          // row by row: lane r finds the address of key r
           const int r_lane = lane & (KT - 1);
           const int64_t row_at = key_span ? at + (int64_t)(r_lane - key_lane) * cache.slot_stride * (Q8 ? 1 : 2) : at;
-          const uint32_t rows = __ballot_sync(ALL, there && key + r_lane >= from && key + r_lane < to);
-#pragma unroll 4
+          const bool row_there = there && key + r_lane >= from && key + r_lane < to;
+          row_address[warp][lane] = row_there ? static_cast<const char*>(cache.keys) + row_at : nullptr;
+          __syncwarp();
+          const uint32_t kd = stage + key_to, vd = stage + value_to;
+#pragma unroll
           for (int i = 0; i < S::COPIES; ++i) {
-            const int r = i * S::RPI + row_lane;
-            const int64_t bytes = __shfl_sync(ALL, row_at, r);
-            const bool live = (rows >> r) & 1;
-            const char* src = static_cast<const char*>(cache.keys) + (live ? bytes + piece_lane * 16 : 0);
-            copy16(stage + S::key_at(r, piece_lane), src, live);
-            copy16(stage + S::TILE + S::value_at(r, piece_lane), live ? src + value_delta : src, live);
+            const char* row = row_address[warp][i * S::RPI + row_lane];
+            const char* src = row ? row + piece_lane * 16 : static_cast<const char*>(cache.keys);
+            copy16((kd ^ S::key_xor(i)) + i * 512, src, row != nullptr);
+            copy16((vd ^ S::value_xor(i)) + i * 512, row ? src + value_delta : src, row != nullptr);
           }
         }
         if constexpr (Q8) {
@@ -569,7 +577,7 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
         const int k = key + (key_span ? lane * (key_span + 1) : key_lane);
         batch = 0;
         pages = -1;
-        if (k + key_span >= from && k < to) pages = table[p.page_shift >= 0 ? k >> p.page_shift : k / cache.page_size];
+        if (k + key_span >= from && k < to) pages = table[page_of(k)];
       }
       copies_commit();
     };
@@ -1232,22 +1240,25 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
     uint32_t waiting = crossing;  // units whose last arrival at the level before was here
 #pragma unroll 1
     for (int level = 1; level <= 2 && waiting; ++level) {
-      __threadfence();
+      // (one thread's fence after the barrier covers what the others wrote before it)
       __syncthreads();
       if (warp == 0) {
         int last = 0;
         if ((waiting >> lane) & 1) {
+          __threadfence();
           const int members = level == 1 ? min(size, ctas - set * size) : sets;
           uint32_t* const ticket = p.ws.tickets + (level - 1) * 2 * MAX_CTAS + cta_slot(c0, level == 1 ? set * size : 0) - MAX_WARPS;
           last = level == 1 || sets > 1 ? atomicAdd(ticket, 1u) + 1 == (uint32_t)members : 0;
-          if (last) *ticket = 0;
+          if (last) {
+            *ticket = 0;
+            __threadfence();
+          }
         }
         const uint32_t arrived = __ballot_sync(ALL, last);
         if (lane == 0) arrived_last = arrived;
       }
       __syncthreads();
       waiting = arrived_last;
-      __threadfence();
 #pragma unroll 1
       for (uint32_t todo_groups = waiting; todo_groups; todo_groups &= todo_groups - 1) {
         const int x = __ffs(todo_groups) - 1;
