@@ -2,8 +2,8 @@
 // rounded to the input type or quantised to e4m3 with a scale per row or per 128 columns.
 //
 // Bound by memory: one pass, the row stays in registers between the sum of squares and the output.
-// A row belongs to one CTA, or to one warp where a warp's registers hold it, so that short rows pay
-// no block barrier. Each lane holds N items of P values: P consecutive ones in a 16-byte piece
+// A row belongs to one CTA, to one warp where a warp's registers hold it (short rows pay no block
+// barrier), or to the 8 or 16 lanes of a warp that it fills. Each lane holds N items of P values: P consecutive ones in a 16-byte piece
 // where rows are aligned, else 4 values 32 columns apart (a warp then still reads consecutive
 // addresses, and an item of a warp is 128 consecutive columns in both layouts of a group).
 
@@ -63,45 +63,57 @@ struct Piece {
   }
 };
 
-// Row statistics over the warps of a row (`warps` of them; 1: no block barrier).
-__device__ __forceinline__ float row_sum(float v, int warps, float* shared) {
+// Row statistics: over the WIDTH lanes of a row, and over its warps where it has several.
+template <int WIDTH>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  if (warps == 1) return v;
-  if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = (threadIdx.x & 31) < warps ? shared[threadIdx.x & 31] : 0.0f;
+  for (int d = WIDTH / 2; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+template <int WIDTH>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+  if constexpr (WIDTH == 32) return __reduce_max_sync(0xffffffffu, v);
 #pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  for (int d = WIDTH / 2; d >= 1; d >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
   return v;
 }
 
+template <int WIDTH>
+__device__ __forceinline__ float row_sum(float v, int warps, float* shared) {
+  v = lanes_sum<WIDTH>(v);
+  if (WIDTH < 32 || warps == 1) return v;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) shared[threadIdx.x >> 5] = v;
+  __syncthreads();
+  return lanes_sum<32>(lane < warps ? shared[lane] : 0.0f);
+}
+
 // Both at once, behind one barrier.
+template <int WIDTH>
 __device__ __forceinline__ void row_sum_and_max(float& v, uint32_t& top, int warps, float* sums, uint32_t* tops) {
-#pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (warps == 1) return;
+  v = lanes_sum<WIDTH>(v);
+  top = lanes_max<WIDTH>(top);
+  if (WIDTH < 32 || warps == 1) return;
   const int lane = threadIdx.x & 31;
   if (lane == 0) sums[threadIdx.x >> 5] = v, tops[threadIdx.x >> 5] = top;
   __syncthreads();
-  v = lane < warps ? sums[lane] : 0.0f;
-  top = __reduce_max_sync(0xffffffffu, lane < warps ? tops[lane] : 0u);
-#pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  v = lanes_sum<32>(lane < warps ? sums[lane] : 0.0f);
+  top = lanes_max<32>(lane < warps ? tops[lane] : 0u);
 }
 
-// N: items a lane; VEC: 16-byte pieces. blockDim.x = 32 * warps of a row, blockDim.y = rows a CTA
-// (more than one only with one warp a row).
-template <typename T, bool Q8, bool VEC, int N>
+// N: items a lane; VEC: 16-byte pieces; WIDTH: lanes of a row. blockDim.x = WIDTH * warps of a row,
+// blockDim.y = rows a CTA (more than one only with one warp a row, or part of one).
+template <typename T, bool Q8, bool VEC, int N, int WIDTH>
 __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
   constexpr int P = VEC ? Piece<T>::P : 4;
   __shared__ float sums[MAX_WARPS];
   __shared__ uint32_t tops[MAX_WARPS];
   grid_dependency_trigger();
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-  if (row >= a.rows) return;  // whole warps: a CTA with several rows has one warp a row
-  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (WIDTH == 32 && row >= a.rows) return;  // whole warps: a CTA with several rows has one warp a row
+  // lanes past the last row share a warp with it: they take part, and hold no columns
+  const int hidden = WIDTH == 32 || row < a.rows ? a.hidden : 0;
+  const int warps = WIDTH == 32 ? blockDim.x >> 5 : 1, warp = WIDTH == 32 ? threadIdx.x >> 5 : 0, lane = threadIdx.x & (WIDTH - 1);
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
   const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
   const T* weight = static_cast<const T*>(a.weight);
@@ -120,7 +132,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       xs[i] = rs[i] = make_uint4(0, 0, 0, 0);
-      if (column(i, 0) < a.hidden) {
+      if (column(i, 0) < hidden) {
         xs[i] = *reinterpret_cast<const uint4*>(x + column(i, 0));
         if (res) rs[i] = *reinterpret_cast<const uint4*>(res + column(i, 0));
       }
@@ -141,7 +153,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
 #pragma unroll
       for (int j = 0; j < P; ++j) {
         const int at = column(i, j);
-        r[i][j] = at < a.hidden ? to_float(x[at]) + (res ? to_float(res[at]) : 0.0f) : 0.0f;
+        r[i][j] = at < hidden ? to_float(x[at]) + (res ? to_float(res[at]) : 0.0f) : 0.0f;
       }
   }
   float sum = 0.0f;
@@ -156,11 +168,11 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if constexpr (VEC) {
-        if (column(i, 0) < a.hidden) *reinterpret_cast<uint4*>(res_out + column(i, 0)) = Piece<T>::pack(r[i]);
+        if (column(i, 0) < hidden) *reinterpret_cast<uint4*>(res_out + column(i, 0)) = Piece<T>::pack(r[i]);
       } else {
 #pragma unroll
         for (int j = 0; j < P; ++j)
-          if (column(i, j) < a.hidden) res_out[column(i, j)] = from_float<T>(r[i][j]);
+          if (column(i, j) < hidden) res_out[column(i, j)] = from_float<T>(r[i][j]);
       }
     }
   }
@@ -170,29 +182,29 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
     if constexpr (VEC) {
       float w[P];
       uint4 ws = make_uint4(0, 0, 0, 0);
-      if (column(i, 0) < a.hidden) ws = __ldg(reinterpret_cast<const uint4*>(weight + column(i, 0)));
+      if (column(i, 0) < hidden) ws = __ldg(reinterpret_cast<const uint4*>(weight + column(i, 0)));
       Piece<T>::unpack(ws, w);
 #pragma unroll
-      for (int j = 0; j < P; ++j) r[i][j] = column(i, 0) < a.hidden ? r[i][j] * w[j] : 0.0f;
+      for (int j = 0; j < P; ++j) r[i][j] = column(i, 0) < hidden ? r[i][j] * w[j] : 0.0f;
     } else {
 #pragma unroll
-      for (int j = 0; j < P; ++j) r[i][j] = column(i, j) < a.hidden ? r[i][j] * to_float(weight[column(i, j)]) : 0.0f;
+      for (int j = 0; j < P; ++j) r[i][j] = column(i, j) < hidden ? r[i][j] * to_float(weight[column(i, j)]) : 0.0f;
     }
   }
 
   if constexpr (!Q8) {
-    const float rstd = __frsqrt_rn(__fdiv_rn(row_sum(sum, warps, sums), (float)a.hidden) + a.eps);
+    const float rstd = __frsqrt_rn(__fdiv_rn(row_sum<WIDTH>(sum, warps, sums), (float)a.hidden) + a.eps);
     T* out = static_cast<T*>(a.out) + row * a.out_stride;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
 #pragma unroll
       for (int j = 0; j < P; ++j) r[i][j] *= rstd;
       if constexpr (VEC) {
-        if (column(i, 0) < a.hidden) *reinterpret_cast<uint4*>(out + column(i, 0)) = Piece<T>::pack(r[i]);
+        if (column(i, 0) < hidden) *reinterpret_cast<uint4*>(out + column(i, 0)) = Piece<T>::pack(r[i]);
       } else {
 #pragma unroll
         for (int j = 0; j < P; ++j)
-          if (column(i, j) < a.hidden) out[column(i, j)] = from_float<T>(r[i][j]);
+          if (column(i, j) < hidden) out[column(i, j)] = from_float<T>(r[i][j]);
       }
     }
   } else {
@@ -218,18 +230,18 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
       for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int j = 0; j < P; ++j) top = max(top, magnitude_bits(r[i][j]));
-      row_sum_and_max(sum, top, warps, sums, tops);
+      row_sum_and_max<WIDTH>(sum, top, warps, sums, tops);
       rstd = __frsqrt_rn(__fdiv_rn(sum, (float)a.hidden) + a.eps);
       scale_of(top);
-      if (threadIdx.x == 0) a.scales[row] = scale;
+      if (threadIdx.x == 0 && hidden) a.scales[row] = scale;
     } else {
-      rstd = __frsqrt_rn(__fdiv_rn(row_sum(sum, warps, sums), (float)a.hidden) + a.eps);
+      rstd = __frsqrt_rn(__fdiv_rn(row_sum<WIDTH>(sum, warps, sums), (float)a.hidden) + a.eps);
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (a.group) {
         // the item's 128 columns: 128 / P neighbouring lanes (the whole warp in the strided layout)
-        constexpr int LANES = VEC ? 128 / P : 32;
+        constexpr int LANES = VEC && 128 / P < WIDTH ? 128 / P : WIDTH;
         uint32_t t = 0;
 #pragma unroll
         for (int j = 0; j < P; ++j) t = max(t, magnitude_bits(r[i][j]));
@@ -237,10 +249,10 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
         for (int d = LANES / 2; d >= 1; d >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, d));
         scale_of(t);
         const int at = VEC ? column(i, 0) : (i * warps + warp) * 128;
-        if (at < a.hidden && lane % LANES == 0) a.scales[row * ((a.hidden + 127) / 128) + at / 128] = scale;
+        if (at < hidden && lane % LANES == 0) a.scales[row * ((a.hidden + 127) / 128) + at / 128] = scale;
       }
       if constexpr (VEC) {
-        if (column(i, 0) < a.hidden) {
+        if (column(i, 0) < hidden) {
           const uint32_t lo = e4m3_pack4(r[i][0] * factor, r[i][1] * factor, r[i][2] * factor, r[i][3] * factor);
           if constexpr (P == 8) {
             const uint32_t hi = e4m3_pack4(r[i][4] * factor, r[i][5] * factor, r[i][6] * factor, r[i][7] * factor);
@@ -252,7 +264,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
       } else {
 #pragma unroll
         for (int j = 0; j < P; ++j)
-          if (column(i, j) < a.hidden) out[column(i, j)] = (uint8_t)e4m3_pack2(r[i][j] * factor, 0.0f);
+          if (column(i, j) < hidden) out[column(i, j)] = (uint8_t)e4m3_pack2(r[i][j] * factor, 0.0f);
       }
     }
   }
@@ -268,15 +280,21 @@ sonic_status run(const SonicResidualNormArgs& a, cudaStream_t stream) {
   n = n == 3 ? 4 : n;
   while ((items + n - 1) / n > MAX_WARPS) n *= 2;
   const int warps = (items + n - 1) / n;
-  const int rows = warps == 1 ? std::min(a.rows, 4) : 1;
-  const dim3 block(32 * warps, rows), grid((a.rows + rows - 1) / rows);
+  int width = 32;
+  if (VEC && warps == 1 && a.hidden <= PER_WARP / 2) width = a.hidden <= PER_WARP / 4 ? 8 : 16;
+  const int rows = warps > 1 ? 1 : width < 32 ? 128 / width : std::min(a.rows, 4);  // whole warps
+  const dim3 block(width * warps, rows), grid((a.rows + rows - 1) / rows);
   const bool pdl = a.flags & SONIC_FLAG_PDL;
   const auto go = [&](auto kernel) { return launch_status(launch_kernel(kernel, grid, block, 0, stream, pdl, 1, a)); };
+  if constexpr (VEC) {
+    if (width == 8) return go(norm_kernel<T, Q8, VEC, 1, 8>);
+    if (width == 16) return go(norm_kernel<T, Q8, VEC, 1, 16>);
+  }
   switch (n) {
-    case 1: return go(norm_kernel<T, Q8, VEC, 1>);
-    case 2: return go(norm_kernel<T, Q8, VEC, 2>);
-    case 4: return go(norm_kernel<T, Q8, VEC, 4>);
-    default: return go(norm_kernel<T, Q8, VEC, 8>);
+    case 1: return go(norm_kernel<T, Q8, VEC, 1, 32>);
+    case 2: return go(norm_kernel<T, Q8, VEC, 2, 32>);
+    case 4: return go(norm_kernel<T, Q8, VEC, 4, 32>);
+    default: return go(norm_kernel<T, Q8, VEC, 8, 32>);
   }
 }
 
