@@ -29,6 +29,16 @@
 //   scale vs multiplies the softmax weight, and m follows u_j + log2 vs_j, so that the fp16 weights
 //   keep their precision whatever the scales. Codes become fp16 exactly; query rows are brought to
 //   fp16's range by a power of two.
+//
+// Measured (device time, head_dim 128, 4 query heads a kv head unless named): 128 requests of 2048 to
+// 16384 keys, e4m3 cache, one token each 302 us (6.2 TB/s of the cache's bytes); 64 requests of 1 to
+// 8192 keys, bf16, 52 us (5.0); 2 requests of 100003 and 131072 keys, 8 query heads, e4m3, 89 us (5.4);
+// one request of 700 keys 7.5 us: launch, one trip to memory and the join over the cluster. With many
+// query rows the products' latency bounds it, not the memory: two warps a scheduler hold all of its
+// registers, and a tile of 16 keys takes a warp some 3000 cycles at 24 rows, 1500 of them the matrix
+// instructions' of both warps. 32 requests of up to 4097 keys, 1 to 5 tokens, bf16, 33 us (2.0 TB/s);
+// 32 requests of 100 to 8192 keys, 4 tokens of 8 query heads, e4m3, 89 us (1.4). Skipping the column
+// tiles that a request's rows do not fill left both as they were: the longest shares are full ones.
 
 #pragma once
 
@@ -43,7 +53,7 @@ namespace {
 
 constexpr int NT_THREADS = 32 * WARPS;
 constexpr int QUEUE = 8;   // pieces a warp's copies may be ahead of its products
-constexpr int START = 3;   // cost of a unit beside its tiles, in tiles
+constexpr int START = 6;   // cost of a unit beside its tiles, in tiles (3: 32 requests of 4 x 8 query rows, e4m3, 94 us for 89)
 constexpr int LEAST = 4;   // cost of a warp's share at least
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -737,7 +747,7 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
 
       // ---- softmax weights ----
       const bool masked = key0 < all_from || key0 + KT > all_to;
-      float vs[MK][2], lv[MK][2];  // value scale of keys g, g + 8, and its logarithm
+      [[maybe_unused]] float vs[MK][2], lv[MK][2];  // value scale of keys g, g + 8, and its logarithm
 #pragma unroll
       for (int m = 0; m < MK; ++m)
 #pragma unroll

@@ -239,7 +239,7 @@ int log2_of(int v) {
   return l;
 }
 
-// As many tokens a CTA as its threads take with APPEND_ITEMS pieces each (one at least, in several rounds of
+// As many tokens a CTA as its threads take with `items` pieces each (one at least, in several rounds of
 // CTAs where a token has more); a small call's are spread over more CTAs.
 Work work_of(int tokens, int heads, int lanes, int items) {
   Work w;
