@@ -176,7 +176,7 @@ struct Shape {
   static constexpr int CPR = ROW / 16;          // 16-byte pieces of it
   static constexpr int RPI = 32 / CPR;          // rows one copy instruction of a warp covers
   // keys of a tile: 4 KB of rows, or 16 (where the accumulators of many query rows fill the registers)
-  static constexpr int KT = Q8 && D == 128 && NT > 2 ? 16 : imin(32, imax(16, 4096 / ROW));
+  static constexpr int KT = Q8 && D == 128 && NT > 3 ? 16 : imin(32, imax(16, 4096 / ROW));
   static constexpr int MK = KT / 16;
   static constexpr int DT = D / 16;
   static constexpr int TILE = KT * ROW;
@@ -185,7 +185,7 @@ struct Shape {
   static constexpr int ROWS = 8 * NT;
   // query fragments stay in registers while they and the accumulators take at most 150 of them
   // (beside e4m3 codes on their way to fp16, 50)
-  static constexpr bool Q_REGISTERS = NT * DT * 6 <= (Q8 ? 50 : 150);
+  static constexpr bool Q_REGISTERS = NT * DT * 6 <= 50;
   static constexpr int Q_BYTES = Q_REGISTERS ? 0 : NT * DT * 256;  // per warp
   // two CTAs an SM share its 227 KB; 16-bit rows of 256 take one CTA
   static constexpr int BUDGET = (!Q8 && D == 256 ? 54 : 27) * 1024;
@@ -304,6 +304,7 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
   __shared__ alignas(16) float2 ring_stats[WARPS][PART_ROWS];
   __shared__ alignas(16) float2 cta_stats[PART_ROWS];  // of a unit's parts in this CTA, joined
   __shared__ uint32_t arrived_last;
+  __shared__ alignas(8) float query_back[WARPS][PART_ROWS];
   __shared__ const char* row_address[WARPS][32];  // key rows of a tile that is copied row by row
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;  // fragment row, and pair of columns
@@ -593,14 +594,16 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
     };
 
     // ---- the products' side ----
-    Piece u;
-    int limit[NT][2];        // last key that query columns 2t and 2t + 1 see
-    float row_scale[NT][2];  // e4m3: undoes the power of two of the query row
+    Piece u{};
+    // e4m3: undoes the power of two of query columns 2t and 2t + 1 (many: in shared memory)
+    float row_scale[S::Q_REGISTERS ? NT : 1][2];
     uint32_t qf[S::Q_REGISTERS ? NT : 1][S::Q_REGISTERS ? DT : 1][2];
     float o[DT][NT][4], ref[NT][2], sum[NT][2];
     int u_from = 0, u_to = 0, all_from = 0, all_to = 0, first_limit = 0, last_limit = 0;
     int stage_out = 0, todo = 0, taken = 0;
 
+    // last key that query column `col` sees
+    const auto limit = [&](int col) { return col < u.rows ? u.offset + token_of(u.row0 + col) : -1; };
     const auto begin_piece = [&]() {
       u = queue[warp][taken % QUEUE];
       ++taken;
@@ -662,11 +665,11 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
           else
             asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(q_smem + ((n * DT + k) * 32 + lane) * 8), "r"(raw[n][k].x), "r"(raw[n][k].y));
         }
+        if constexpr (Q8 && !S::Q_REGISTERS)
+          if (t == 0) query_back[warp][n * 8 + g] = back;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int col = n * 8 + 2 * t + c;
-          limit[n][c] = col < u.rows ? u.offset + token_of(u.row0 + col) : -1;
-          row_scale[n][c] = Q8 ? __shfl_sync(ALL, back, (2 * t + c) * 4) : 1.0f;
+          if constexpr (Q8 && S::Q_REGISTERS) row_scale[n][c] = __shfl_sync(ALL, back, (2 * t + c) * 4);
           ref[n][c] = -INFINITY;
           sum[n][c] = 0.0f;
         }
@@ -747,6 +750,18 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
 
       // ---- softmax weights ----
       const bool masked = key0 < all_from || key0 + KT > all_to;
+      [[maybe_unused]] float back[NT][2];
+      if constexpr (Q8) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if constexpr (S::Q_REGISTERS) {
+            back[n][0] = row_scale[n][0], back[n][1] = row_scale[n][1];
+          } else {
+            const uint2 v = load_shared8(shared_address(query_back[warp] + n * 8 + 2 * t));
+            back[n][0] = __uint_as_float(v.x), back[n][1] = __uint_as_float(v.y);
+          }
+        }
+      }
       [[maybe_unused]] float vs[MK][2], lv[MK][2];  // value scale of keys g, g + 8, and its logarithm
 #pragma unroll
       for (int m = 0; m < MK; ++m)
@@ -766,7 +781,7 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
               float v = s[m][n][2 * h + c] * ks;
-              if constexpr (Q8) v *= row_scale[n][c];
+              if constexpr (Q8) v *= back[n][c];
               s[m][n][2 * h + c] = v;
             }
         }
@@ -777,7 +792,7 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int key = key0 + m * 16 + g + 8 * (i >> 1), l = limit[n][i & 1];
+              const int key = key0 + m * 16 + g + 8 * (i >> 1), l = limit(n * 8 + 2 * t + (i & 1));
               if (key > l || (p.window && key <= l - p.window)) s[m][n][i] = -INFINITY;
             }
       }
@@ -909,7 +924,7 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
               for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                  if (limit[n][i & 1] == l) reinterpret_cast<float*>(acc + j * NT + n)[i] = x[n][i];
+                  if (limit(n * 8 + 2 * t + (i & 1)) == l) reinterpret_cast<float*>(acc + j * NT + n)[i] = x[n][i];
             }
           }
 #pragma unroll
@@ -1064,14 +1079,17 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
     copies_wait<0>();
 
     // ---- units that several warps share ----
-    // Join n_parts parts of piece x, in order: row tiles j0, j0 + step, ... (J at most), P parts' loads in
-    // flight at once. stats(k, i) and values(k, i) give float4 i of part k; into the output, or to
-    // `stats_to` and `values_to`.
-    const auto join = [&](auto jc, auto pc, const Piece& x, int n_parts, int j0, int step, auto&& stats, auto&& values, bool out,
-                          float4* stats_to, float4* values_to) {
-      constexpr int J = decltype(jc)::value, P = decltype(pc)::value;
-#pragma unroll 1
-      for (int n = 0; n < NT && n * 8 < x.rows; ++n) {
+    // Join n_parts parts of piece x, in order, as warp `member` of `members`: one of the column tiles,
+    // and of its row tiles j0, j0 + step, ... (J at most), with P parts' loads in flight at once. (A warp
+    // for each column tile, not each in turn: those are trips to memory one after the other.)
+    // stats(k, i) and values(k, i) give float4 i of part k; into the output, or to `stats_to` and
+    // `values_to`.
+    constexpr int SIDE = NT > 2 ? 4 : NT;
+    const auto join = [&](auto jc, auto pc, const Piece& x, int n_parts, int member, int members, auto&& stats, auto&& values,
+                          bool out, float4* stats_to, float4* values_to) {
+      constexpr int J = decltype(jc)::value, P = imin(decltype(pc)::value, imax(1, 16 / J));
+      const int n = member % SIDE, j0 = member / SIDE, step = members / SIDE;
+      if (n < NT && n * 8 < x.rows) {
         const int col = n * 8 + 2 * t;
         const bool live = col < x.rows;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
@@ -1130,8 +1148,8 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
         }
       }
     };
-    using PerWarp = std::integral_constant<int, (DT + WARPS - 1) / WARPS>;  // row tiles of a warp of the CTA
-    using PerClusterWarp = std::integral_constant<int, imax(1, DT / 8)>;  // of 8 warps or more
+    using PerWarp = std::integral_constant<int, imax(1, DT * SIDE / WARPS)>;  // row tiles of a warp of the CTA
+    using PerClusterWarp = std::integral_constant<int, imax(1, DT * SIDE / 8)>;  // of 8 warps or more
     using Few = std::integral_constant<int, WARPS>;
     using Many = std::integral_constant<int, 8>;
 
