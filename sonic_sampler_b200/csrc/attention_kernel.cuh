@@ -1316,16 +1316,16 @@ sonic_status launch_attention(const AttentionLaunch& launch, cudaStream_t stream
   const int64_t row_tiles = ((int64_t)p.most * p.group + S::ROWS - 1) / S::ROWS;
   const int64_t units = (int64_t)s.requests * p.a.cache.kv_heads * row_tiles;
   // A fixed number of warps a unit where that leaves a warp at most 16 tiles of the longest possible
-  // one, in up to two waves of CTAs, or 32 in at least half a wave and at most one: there the balanced
-  // shares' scan and joins cost more than uneven lengths do. (us, fixed against balanced: 37 requests of
-  // 1024 keys, 8 kv heads, bf16: 29 against 36; 64 of up to 1000, 4 queries: 34 against 37; 32 of up to
-  // 4097, 5 queries, which would take 1024 CTAs: 49 against 33.)
+  // one and the CTAs run at once (of one warp a unit, in two waves): there the balanced shares' scan
+  // and joins cost more than uneven lengths do. (us, fixed against balanced, 8 kv heads, bf16: 37
+  // requests of 512 keys 17 against 24, 32 of 1000 26 against 31, of 1 to 1000 16 against 14. Beyond
+  // these limits: 32 of 2000 45 against 52, but of 1 to 2000 27 against 18; 64 of 1 to 1000 with 4
+  // queries, which take two waves, 28 against 23.)
   const int64_t tiles = ((p.window ? std::min<int64_t>(p.room, (int64_t)p.window + p.most) : p.room) + S::KT - 1) / S::KT + 1;
   const auto ctas_of = [&](int warps) { return (units * warps + WARPS - 1) / WARPS; };
   const auto more = [](int warps) { return warps == 1 ? WARPS : 2 * warps; };
   const auto fits = [&](int warps) {
-    const int64_t ctas = ctas_of(warps);
-    return (tiles <= 16 * warps && ctas <= 2 * S::CTAS) || (tiles <= 32 * warps && 2 * ctas >= S::CTAS && ctas <= S::CTAS);
+    return tiles <= 16 * warps && ctas_of(warps) <= (warps == 1 ? 2 : 1) * S::CTAS;
   };
   p.unit_warps = 1;
   while (p.unit_warps < 32 && !fits(p.unit_warps)) p.unit_warps = more(p.unit_warps);
