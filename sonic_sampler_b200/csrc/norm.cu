@@ -7,10 +7,11 @@
 // where rows are aligned, else 4 values 32 columns apart (a warp then still reads consecutive
 // addresses, and an item of a warp is 128 consecutive columns in both layouts of a group).
 //
-// bf16 with a residual to e4m3, device time: 16384 x 8192 137 us with a scale a row, 150 us a scale per
-// 128 columns (6.9 and 6.3 TB/s of the bytes that it has to move); 64 x 4096 2.7 us, launch and one
-// trip to memory. 32768 x 128, 16 lanes a row, 7.5 us (a warp a row: 12.0). The strided layout is bound
-// by instructions, some 30 a value: 3000 x 5001 takes 30 us, twice what its bytes would.
+// bf16 with a residual to e4m3, device time: 16384 x 8192 138 us with a scale a row, 141 us a scale per
+// 128 columns (6.8 and 6.7 TB/s of the bytes that it has to move); 64 x 4096 2.7 us, launch and one
+// trip to memory. 32768 x 128, 16 lanes a row, 7.4 us (a warp a row: 12.0). The strided layout is bound
+// by instructions, some 30 a value: 3000 x 5001 takes 30 us, twice what its bytes would. With a
+// division and a maximum by bits for every 128 columns in every lane those were 141 -> 150 us and 31 -> 36.
 
 #include <algorithm>
 
@@ -67,6 +68,16 @@ struct Piece {
       return make_uint4(Pair<T>::pack(f[0], f[1]), Pair<T>::pack(f[2], f[3]), Pair<T>::pack(f[4], f[5]), Pair<T>::pack(f[6], f[7]));
   }
 };
+
+// Bits of the largest magnitude of v, ordered as magnitude_bits; a NaN is the largest.
+template <int P>
+__device__ __forceinline__ uint32_t largest(const float (&v)[P]) {
+  float top = v[0];
+#pragma unroll
+  for (int j = 1; j < P; j += 2)
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(top) : "f"(top), "f"(v[j]), "f"(v[j + 1 < P ? j + 1 : j]));
+  return magnitude_bits(top);
+}
 
 // Row statistics: over the WIDTH lanes of a row, and over its warps where it has several.
 template <int WIDTH>
@@ -256,6 +267,8 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
     // the scales' floor is mapped by rstd * 448 / floor.
     uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.out_stride;
     float rstd, scale, factor;
+    // an item's 128 columns lie in 128 / P neighbouring lanes (the whole warp in the strided layout)
+    constexpr int LANES = VEC && 128 / P < WIDTH ? 128 / P : WIDTH;
     const auto scale_of = [&](uint32_t top) {
       const float z = __uint_as_float(top), c = z * rstd;
       if (c < kScaleFloor) {
@@ -270,35 +283,35 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
     if (a.group == 0) {
       uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int j = 0; j < P; ++j) top = max(top, magnitude_bits(r[i][j]));
+      for (int i = 0; i < N; ++i) top = max(top, largest(r[i]));
       row_sum_and_max<WIDTH>(sum, top, warps, sums, tops);
       rstd = __frsqrt_rn(__fdiv_rn(sum, (float)a.hidden) + a.eps);
       scale_of(top);
       if (threadIdx.x == 0 && hidden) a.scales[row] = scale;
     } else {
       rstd = __frsqrt_rn(__fdiv_rn(row_sum<WIDTH>(sum, warps, sums), (float)a.hidden) + a.eps);
+      // lane i of an item's lanes finds the scale and factor of item i: one division each, not one an item
+      const int member = lane % LANES;
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        uint32_t t = largest(r[i]);
+#pragma unroll
+        for (int d = LANES / 2; d >= 1; d >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, d));
+        if (member == i) top = t;
+      }
+      scale_of(top);
+      const int at = VEC ? column(member, 0) - member * P : (member * warps + warp) * 128;
+      if (member < N && at < hidden) a.scales[row * ((a.hidden + 127) / 128) + at / 128] = scale;
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (a.group) {
-        // the item's 128 columns: 128 / P neighbouring lanes (the whole warp in the strided layout)
-        constexpr int LANES = VEC && 128 / P < WIDTH ? 128 / P : WIDTH;
-        uint32_t t = 0;
-#pragma unroll
-        for (int j = 0; j < P; ++j) t = max(t, magnitude_bits(r[i][j]));
-#pragma unroll
-        for (int d = LANES / 2; d >= 1; d >>= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, d));
-        scale_of(t);
-        const int at = VEC ? column(i, 0) : (i * warps + warp) * 128;
-        if (at < hidden && lane % LANES == 0) a.scales[row * ((a.hidden + 127) / 128) + at / 128] = scale;
-      }
+      const float f = a.group ? __shfl_sync(0xffffffffu, factor, i, LANES) : factor;
       if constexpr (VEC) {
         if (column(i, 0) < hidden) {
-          const uint32_t lo = e4m3_pack4(r[i][0] * factor, r[i][1] * factor, r[i][2] * factor, r[i][3] * factor);
+          const uint32_t lo = e4m3_pack4(r[i][0] * f, r[i][1] * f, r[i][2] * f, r[i][3] * f);
           if constexpr (P == 8) {
-            const uint32_t hi = e4m3_pack4(r[i][4] * factor, r[i][5] * factor, r[i][6] * factor, r[i][7] * factor);
+            const uint32_t hi = e4m3_pack4(r[i][4] * f, r[i][5] * f, r[i][6] * f, r[i][7] * f);
             *reinterpret_cast<uint2*>(out + column(i, 0)) = make_uint2(lo, hi);
           } else {
             *reinterpret_cast<uint32_t*>(out + column(i, 0)) = lo;
@@ -306,7 +319,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
         }
       } else {
         uint8_t* to = out + column(i, 0);
-        const uint32_t codes = e4m3_pack4(r[i][0] * factor, r[i][1] * factor, r[i][2] * factor, r[i][3] * factor);
+        const uint32_t codes = e4m3_pack4(r[i][0] * f, r[i][1] * f, r[i][2] * f, r[i][3] * f);
         if (whole(i)) {
 #pragma unroll
           for (int j = 0; j < P; ++j) to[32 * j] = codes >> 8 * j;
