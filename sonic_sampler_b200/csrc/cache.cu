@@ -40,14 +40,15 @@ __device__ __forceinline__ Slot find_slot(const SonicPagedCache& c, const SonicS
                                           uint32_t* error) {
   Slot found;
   if (position < 0) return found;
-  const int64_t index = position / c.page_size;
+  // (a position is below some int32 length: a 32-bit division will do)
+  const uint32_t index = (uint32_t)position / (uint32_t)c.page_size;
   int page = -1;
-  if (index < s.table_width) page = s.page_table[request * s.table_stride + index];
+  if (index < (uint32_t)s.table_width) page = s.page_table[request * s.table_stride + index];
   if (page < 0 || page >= c.pages) {
     if (error) atomicOr(error, (uint32_t)SONIC_DEVICE_ERR_PAGE);
     return found;
   }
-  const int slot = (int)(position - index * c.page_size);
+  const int slot = (int)((uint32_t)position - index * (uint32_t)c.page_size);
   found.at = page * c.page_stride + slot * c.slot_stride;
   found.scale = page * c.scale_page_stride + slot;
   return found;
