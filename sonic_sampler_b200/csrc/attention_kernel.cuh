@@ -36,9 +36,9 @@
 // one request of 700 keys 7.5 us: launch, one trip to memory and the join over the cluster. With many
 // query rows the products' latency bounds it, not the memory: two warps a scheduler hold all of its
 // registers, and a tile of 16 keys takes a warp some 3000 cycles at 24 rows, 1500 of them the matrix
-// instructions' of both warps. 32 requests of up to 4097 keys, 1 to 5 tokens, bf16, 33 us (2.0 TB/s);
-// 32 requests of 100 to 8192 keys, 4 tokens of 8 query heads, e4m3, 89 us (1.4). Skipping the column
-// tiles that a request's rows do not fill left both as they were: the longest shares are full ones.
+// instructions' of both warps. 32 requests of up to 4097 keys, 1 to 5 tokens, bf16, 27 us (2.4 TB/s);
+// 32 requests of 100 to 8192 keys, 4 tokens of 8 query heads, e4m3, 67 us (1.9). Skipping the column
+// tiles that a request's rows do not fill changes neither: the longest shares are full ones.
 
 #pragma once
 
@@ -175,7 +175,8 @@ struct Shape {
   static constexpr int ROW = D * (Q8 ? 1 : 2);  // bytes of a cached row
   static constexpr int CPR = ROW / 16;          // 16-byte pieces of it
   static constexpr int RPI = 32 / CPR;          // rows one copy instruction of a warp covers
-  // keys of a tile: 4 KB of rows, or 16 (where the accumulators of many query rows fill the registers)
+  // keys of a tile: 4 KB of rows, or 16 where four column tiles' accumulators fill the registers (32 keys:
+  // 82 us against 78; at three column tiles 49 against 54 with 16)
   static constexpr int KT = Q8 && D == 128 && NT > 3 ? 16 : imin(32, imax(16, 4096 / ROW));
   static constexpr int MK = KT / 16;
   static constexpr int DT = D / 16;
@@ -183,8 +184,9 @@ struct Shape {
   static constexpr int COPIES = TILE / 512;     // copy instructions of a tile
   static constexpr int STAGE = 2 * TILE + (Q8 ? imax(2 * KT * 4, 128) : 0);  // keys, values, their scales
   static constexpr int ROWS = 8 * NT;
-  // query fragments stay in registers while they and the accumulators take at most 150 of them
-  // (beside e4m3 codes on their way to fp16, 50)
+  // query fragments stay in registers while they and the accumulators take at most 50 of them; beyond,
+  // the registers do more for the products in flight (head_dim 128, three column tiles, bf16: 27 us
+  // against 33)
   static constexpr bool Q_REGISTERS = NT * DT * 6 <= 50;
   static constexpr int Q_BYTES = Q_REGISTERS ? 0 : NT * DT * 256;  // per warp
   // two CTAs an SM share its 227 KB; 16-bit rows of 256 take one CTA
