@@ -420,6 +420,33 @@ def load_library(path: os.PathLike | str | None = None) -> ctypes.CDLL:
     return lib
 
 
+_CALLS = None
+
+
+def load_calls():
+    """Load (once) and return the CPython module of the decode-side calls, bound to the CUDA library's
+    entry points. Raises RuntimeError when it is not built for the installed torch."""
+    global _CALLS
+    if _CALLS is None:
+        import importlib.machinery
+        import importlib.util
+
+        from sonic_sampler_b200.build import calls_path
+
+        lib, path = load_library(), calls_path()
+        if not path.is_file():
+            raise RuntimeError(f"{path} is missing: build it first (python -m sonic_sampler_b200.build, or __graft_entry__.build())")
+        loader = importlib.machinery.ExtensionFileLoader("sonic_b200_calls", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("sonic_b200_calls", loader))
+        loader.exec_module(module)
+        if module.abi_version != ABI_VERSION:
+            raise RuntimeError(f"{path} has ABI {module.abi_version}, expected {ABI_VERSION}")
+        module.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            lib.sonic_residual_norm, lib.sonic_cache_append, lib.sonic_cache_gather, lib.sonic_paged_attention)))
+        _CALLS = module
+    return _CALLS
+
+
 class SonicError(RuntimeError):
     """A C-ABI call returned a non-zero status."""
 

@@ -3,7 +3,8 @@
     python -m sonic_sampler_b200.build [--force]
 
 nvcc cross-compiles without a GPU. The library links the CUDA runtime statically, so it
-only needs the driver at run time.
+only needs the driver at run time. Beside it lies the CPython module of `csrc/calls.cpp`, which is
+built for the installed torch.
 """
 
 from __future__ import annotations
@@ -19,6 +20,7 @@ PACKAGE_DIR = Path(__file__).resolve().parent
 CSRC = PACKAGE_DIR / "csrc"
 OUT = PACKAGE_DIR / "_lib" / "libsonic_b200.so"
 # diagnostic variant with per-phase timing stamps (python -m sonic_sampler_b200.phases)
+CALLS = CSRC / "calls.cpp"
 STAMPS_OUT = PACKAGE_DIR / "_lib" / "libsonic_b200_stamps.so"
 API = PACKAGE_DIR.parent / "include" / "sonic_b200.h"
 EXPORTS = CSRC / "exports.map"
@@ -62,17 +64,39 @@ def nvcc_path() -> str:
     raise RuntimeError("nvcc not found (set CUDA_HOME or put nvcc on PATH)")
 
 
-def stale(out: Path = OUT) -> bool:
+def stale(out: Path = OUT, sources: list[Path] = SOURCES + HEADERS) -> bool:
     if not out.is_file():
         return True
     t = out.stat().st_mtime
-    return any(p.stat().st_mtime > t for p in SOURCES + HEADERS)
+    return any(p.stat().st_mtime > t for p in sources)
+
+
+def calls_path() -> Path:
+    """The CPython module for the torch that is installed (its C++ classes differ between versions)."""
+    import torch
+
+    return PACKAGE_DIR / "_lib" / f"sonic_b200_calls_{torch.__version__}.so"
+
+
+def calls_command() -> list[str]:
+    import sysconfig
+
+    import torch
+
+    home = Path(torch.__file__).resolve().parent
+    includes = [home / "include", home / "include" / "torch" / "csrc" / "api" / "include",
+                Path(nvcc_path()).resolve().parents[1] / "include", sysconfig.get_paths()["include"]]
+    return [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in includes), str(CALLS),
+            f"-L{home / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
 
 
 def build(force: bool = False, verbose: bool = False, stamps: bool = False) -> Path:
     """Build the product library, or with `stamps` the phase-stamp diagnostic variant."""
     out = STAMPS_OUT if stamps else OUT
-    if not force and not stale(out):
+    calls = calls_path()
+    fresh_calls = not force and not stale(calls, [CALLS, API])
+    if fresh_calls and not stale(out):
         return out
     out.parent.mkdir(parents=True, exist_ok=True)
     define = ["-DSONIC_PHASE_STAMPS"] if stamps else []
@@ -85,6 +109,8 @@ def build(force: bool = False, verbose: bool = False, stamps: bool = False) -> P
         newest = max(p.stat().st_mtime for p in (source, *headers, Path(__file__)))
         if force or not obj.is_file() or obj.stat().st_mtime < newest:
             commands.append(([nvcc_path(), *COMPILE_FLAGS, *UNIT_FLAGS.get(source, []), *define, "-c", str(source)], obj))
+    if not fresh_calls:
+        commands.append((calls_command(), calls))
 
     def run(cmd, target):
         tmp = target.with_suffix(target.suffix + ".tmp")

@@ -11,12 +11,13 @@ wrote lies past the new length and is overwritten by the next tokens.
 
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 import torch
 from torch import Tensor
 
-from sonic_sampler_b200 import ops
+from sonic_sampler_b200 import _abi, ops
 from sonic_sampler_b200._abi import FLAG_PDL
 
 E4M3 = torch.float8_e4m3fn
@@ -41,6 +42,9 @@ class PagedCache:
         self.flags = FLAG_PDL if self.pdl else 0
         # the device error word of append and gather
         self.errors = ops.new_workspace(256, self.device)
+        # what `_abi.load_calls()`'s functions take of it
+        self.address = ctypes.addressof(self.struct)
+        self.place = (self.address, self.device.index, self.flags, self.errors.data_ptr())
 
     @classmethod
     def allocate(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
@@ -65,6 +69,9 @@ class PagedCache:
         its largest magnitude and 2^-60, and its codes are rounded to nearest even. Runs on the
         current stream; a token whose page is not in the cache is skipped and recorded
         (`device_error`)."""
+        status = _abi.load_calls().append(*self.place, keys, values, page_table, lengths, cu_seqlens)
+        if status == 0:
+            return self
         ops._require_cuda(keys)
         args = ops.cache_append_args(self.struct, keys, values, page_table, lengths, cu_seqlens=cu_seqlens,
                                      flags=self.flags, error=self.errors, device=self.device)
@@ -79,9 +86,13 @@ class PagedCache:
 
         An e4m3 row is code * scale, rounded once to `dtype` (bf16 by default, or fp16); other caches
         keep their dtype. `keys` and `values` may give the outputs to write."""
-        ops._require_cuda(page_table)
         if dtype is None:
             dtype = keys.dtype if keys is not None else torch.bfloat16 if self.keys.dtype == E4M3 else self.keys.dtype
+        if keys is None and values is None and (dtype == torch.bfloat16 or dtype == torch.float16):
+            rows = _abi.load_calls().gather(*self.place, page_table, starts, total, dtype == torch.float16)
+            if type(rows) is tuple:
+                return rows
+        ops._require_cuda(page_table)
         args, keys, values = ops.cache_gather_args(self.struct, page_table, starts, total, dtype, keys, values, flags=self.flags,
                                                    error=self.errors, device=self.device)
         ops.launch_cache_gather(args, self.device)

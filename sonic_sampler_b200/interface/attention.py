@@ -7,12 +7,13 @@ side of a speculative verification (`UnshardedFusedMultistep` then judges its lo
 
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 import torch
 from torch import Tensor
 
-from sonic_sampler_b200 import ops
+from sonic_sampler_b200 import _abi, ops
 from sonic_sampler_b200._abi import FLAG_PDL
 from sonic_sampler_b200.core.cache import PagedCache
 from sonic_sampler_b200.interface.base import default_device
@@ -30,6 +31,7 @@ class PagedAttention:
 
     def __post_init__(self):
         self.template = ops.paged_attention_template(self.q_heads, self.head_dim, FLAG_PDL if self.pdl else 0)
+        self.address = ctypes.addressof(self.template)
 
     @classmethod
     def initialize(cls, q_heads: int, kv_heads: int, head_dim: int, lookahead: int = 0, pdl: bool = True) -> "PagedAttention":
@@ -62,10 +64,16 @@ class PagedAttention:
         Returns the output (in `output` where that is given), and with `logsumexp` also the fp32
         `[tokens, q_heads]` logarithms of the softmax sums, with which outputs over disjoint key
         ranges can be joined. A query that sees no key gives zeros and -infinity."""
-        ops._require_cuda(queries)
         struct, device, scratchpad = cache.struct, cache.device, self.scratchpad
         if struct.kv_heads != self.kv_heads or struct.head_dim != self.head_dim:
             raise ValueError("the cache's kv_heads and head_dim must match `initialize`'s")
+        if output is None and scratchpad.device == device:
+            found = _abi.load_calls().attention(self.address, cache.address, device.index, scratchpad.data_ptr(), scratchpad.numel(),
+                                                queries, page_table, lengths, cu_seqlens, self.lookahead + 1, window, scale,
+                                                logsumexp)
+            if found is not None and type(found) is not int:
+                return found
+        ops._require_cuda(queries)
         if window is None:
             window = 0
         elif window < 1:
