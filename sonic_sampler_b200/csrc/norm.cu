@@ -69,6 +69,16 @@ struct Piece {
   }
 };
 
+// What the fp32 quotient f = 448 / top leaves of 448 / top, to a few bits: top * (f + rest) = 448. With
+// it z * 448 / top is rounded once on its way to a code, so that quotients of short significands that lie
+// on the midpoint of two codes are seen to lie there. 0 where the row holds an infinity. (It costs nothing
+// that shows here: 16384 x 8192 takes 141 us either way. The cache's append is bound by its instructions
+// and keeps the plain product: 20.7 us against 22.1.)
+__device__ __forceinline__ float e4m3_rest(float top, float f) {
+  return top <= 3.4028235e38f ? fmaf(-f, top, kE4m3Max) * (f * (1.0f / kE4m3Max)) : 0.0f;
+}
+__device__ __forceinline__ float e4m3_quotient(float x, float f, float rest) { return fmaf(x, f, x * rest); }
+
 // Bits of the largest magnitude of v, ordered as magnitude_bits; a NaN is the largest.
 template <int P>
 __device__ __forceinline__ uint32_t largest(const float (&v)[P]) {
@@ -263,10 +273,10 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
     }
   } else {
     // The codes of a row or group do not depend on rstd, which its largest |y| shares: they are
-    // e4m3(z * (448 / max |z|)), one rounding less on the way. Only a row whose largest |y| lies below
+    // e4m3(z * 448 / max |z|), rounded once after z. Only a row whose largest |y| lies below
     // the scales' floor is mapped by rstd * 448 / floor.
     uint8_t* out = static_cast<uint8_t*>(a.out) + row * a.out_stride;
-    float rstd, scale, factor;
+    float rstd, scale, factor, rest;
     // an item's 128 columns lie in 128 / P neighbouring lanes (the whole warp in the strided layout)
     constexpr int LANES = VEC && 128 / P < WIDTH ? 128 / P : WIDTH;
     const auto scale_of = [&](uint32_t top) {
@@ -274,10 +284,12 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
       if (c < kScaleFloor) {
         scale = kScaleFloor / kE4m3Max;
         factor = rstd * (kE4m3Max / kScaleFloor);
+        rest = 0.0f;
       } else {
         scale = __fdiv_rn(c, kE4m3Max);
         // (448 / z would overflow for the tiniest z); a NaN makes the whole row NaN
         factor = !(c == c) ? c : z < kScaleFloor ? rstd * __fdiv_rn(kE4m3Max, c) : __fdiv_rn(kE4m3Max, z);
+        rest = z < kScaleFloor ? 0.0f : e4m3_rest(z, factor);
       }
     };
     if (a.group == 0) {
@@ -307,11 +319,15 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float f = a.group ? __shfl_sync(0xffffffffu, factor, i, LANES) : factor;
+      const float f_rest = a.group ? __shfl_sync(0xffffffffu, rest, i, LANES) : rest;
+      float q[P];
+#pragma unroll
+      for (int j = 0; j < P; ++j) q[j] = e4m3_quotient(r[i][j], f, f_rest);
       if constexpr (VEC) {
         if (column(i, 0) < hidden) {
-          const uint32_t lo = e4m3_pack4(r[i][0] * f, r[i][1] * f, r[i][2] * f, r[i][3] * f);
+          const uint32_t lo = e4m3_pack4(q[0], q[1], q[2], q[3]);
           if constexpr (P == 8) {
-            const uint32_t hi = e4m3_pack4(r[i][4] * f, r[i][5] * f, r[i][6] * f, r[i][7] * f);
+            const uint32_t hi = e4m3_pack4(q[4], q[5], q[6], q[7]);
             *reinterpret_cast<uint2*>(out + column(i, 0)) = make_uint2(lo, hi);
           } else {
             *reinterpret_cast<uint32_t*>(out + column(i, 0)) = lo;
@@ -319,7 +335,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(SonicResidualNormArgs a) {
         }
       } else {
         uint8_t* to = out + column(i, 0);
-        const uint32_t codes = e4m3_pack4(r[i][0] * f, r[i][1] * f, r[i][2] * f, r[i][3] * f);
+        const uint32_t codes = e4m3_pack4(q[0], q[1], q[2], q[3]);
         if (whole(i)) {
 #pragma unroll
           for (int j = 0; j < P; ++j) to[32 * j] = codes >> 8 * j;
