@@ -220,15 +220,63 @@ def config5(device, seed: int = 0, batch: int = 1024, vocab: int = 256000):
     )
 
 
+def paged_tokens(lengths: list[int], page_size: int, device, seed: int) -> tuple[Tensor, Tensor, int]:
+    """(page table, lengths, pages) of requests whose pages lie in no order."""
+    each = [-(-n // page_size) for n in lengths]
+    order = torch.randperm(sum(each), generator=torch.Generator().manual_seed(seed)).to(I32)
+    table = torch.zeros(len(lengths), max(each), dtype=I32)
+    for row, pages in zip(table, order.split(each)):
+        row[: pages.numel()] = pages
+    return table.to(device), torch.tensor(lengths, dtype=I32, device=device), sum(each)
+
+
+def decode_side(name: str, device, pdl: bool = True):
+    """A no-argument callable that runs one operator between two sampler calls once: 8 kv heads and 32 query
+    heads of 128, pages of 16."""
+    from sonic_sampler_b200.interface import PagedAttention, PagedCache, ResidualNorm
+
+    dev, e4m3 = torch.device(device), torch.float8_e4m3fn
+    g = _gen(dev, 5)
+
+    def normal(*shape, dtype=BF16):
+        return torch.randn(shape, generator=g, device=dev, dtype=dtype)
+
+    if name == "residual_norm":
+        x, residual, weight = normal(8192, 8192), normal(8192, 8192), 1.0 + 0.1 * normal(8192)
+        norm = ResidualNorm(weight, dtype=e4m3, group=128, pdl=pdl)
+        return lambda: norm(x, residual)
+    lengths = {"attention_decode": [2048 + 448 * b for b in range(32)], "attention_verify": [1 + 128 * b for b in range(32)],
+               "cache_append": [2500] * 8, "cache_gather": [3000 + 600 * b for b in range(16)]}[name]
+    table, tokens, pages = paged_tokens(lengths, 16, dev, 6)
+    cache = PagedCache.allocate(pages, 16, 8, 128, dtype=BF16 if name == "attention_verify" else e4m3, device=dev, pdl=pdl)
+    starts = torch.nn.functional.pad(tokens.cumsum(0), (1, 0)).to(I32)
+    held = normal(sum(lengths), 2, 8, 128)
+    cache.append(held[:, 0], held[:, 1], table, tokens, starts)
+    if name == "cache_append":
+        new = normal(16000, 2, 8, 128)
+        return lambda: cache.append(new[:, 0], new[:, 1], table, tokens)
+    if name == "cache_gather":
+        return lambda: cache.gather(table, starts, sum(lengths))
+    each = 5 if name == "attention_verify" else 1
+    attention = PagedAttention.initialize(32, 8, 128, lookahead=each - 1, pdl=pdl)
+    queries = normal(32 * each, 32, 128)
+    return lambda: attention(queries, cache, table, tokens)
+
+
+DECODE_SIDE = ("attention_decode", "attention_verify", "cache_append", "cache_gather", "residual_norm")
+
+
 def runner(name: str, device, pdl: bool = True):
     """A no-argument callable that runs benchmark config `name` once through the public
     interface (config 2: UnshardedFusedSingular.autoregressive; 3: fused_multistep; 4: three
     cross-vocabulary greedy drafting steps and a greedy verification, as one chain;
     5: fused_singular with Philox noise; 1: UnshardedBoundedTopK; indexed_copy: the noise
     staging of GumbelNoise.stage_weights; config4_verify[_logits_only]: config 4's verification
-    step alone). `pdl` sets the programmatic-dependent-launch attribute of the sampler launches
+    step alone; the names of DECODE_SIDE: the operators between two sampler calls). `pdl` sets the programmatic-dependent-launch attribute of the sampler launches
     (the interface objects' `pdl`, the functional calls' `enable_pdl`)."""
     dev = torch.device(device)
+    if name in DECODE_SIDE:
+        return decode_side(name, dev, pdl)
     if name == "config1":
         from sonic_sampler_b200.interface import UnshardedBoundedTopK
 
