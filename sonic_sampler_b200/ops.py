@@ -480,10 +480,10 @@ def paged_cache_struct(keys: Tensor, values: Tensor, key_scales: Tensor | None, 
     return c
 
 
-# The builders below run once a call of a decode step, where the host's time shows: messages are
-# formatted only where a check fails, each attribute of a tensor is asked for once, the fields that
-# an interface object never changes come from its template, and outputs that are allocated here
-# need no checks.
+# The builders below take every form of a call's arguments and say what is wrong with them. Calls in
+# the usual form do not come here: `_abi.load_calls()`'s functions (csrc/calls.cpp) fill the same structs.
+# Messages are formatted only where a check fails, each attribute of a tensor is asked for once, and the
+# fields that an interface object never changes come from its template.
 
 
 def _sequences(a, tokens: int, page_table: Tensor, lengths: Tensor | None, cu_seqlens: Tensor | None, device: torch.device) -> int:
