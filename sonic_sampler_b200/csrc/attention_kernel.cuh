@@ -204,6 +204,10 @@ struct Shape {
   // most 2^14, so that small ones stay above fp16's smallest normal
   static constexpr float SLACK = 4.0f;
   static constexpr float SHIFT = std::is_same<M, __half>::value ? 10.0f : 0.0f;
+  // A value scale of zero (or NaN, or a tiny one) counts as 2^LEAST_LOG in m: its key weighs in the sum,
+  // with at most 2^(SLACK + SHIFT - LEAST_LOG) = 2^94, which the 2^30 keys of the longest request keep
+  // below fp32's largest. (Appended rows have scales of 2^-69 and more.)
+  static constexpr float LEAST_LOG = -80.0f;
 
   // byte offset of piece c of key row r, and of value row r: the pieces are permuted so that the
   // fragment reads below are free of bank conflicts. A row further on by RPI i lies 512 i further
@@ -775,8 +779,7 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
             const uint32_t at = stage + 2 * S::TILE + (m * 16 + 8 * h + g) * 4;
             ks *= __uint_as_float(load_shared4(at));
             vs[m][h] = __uint_as_float(load_shared4(at + KT * 4));
-            // (a scale of zero or NaN still leaves its key in the sum)
-            lv[m][h] = fmaxf(log2_fast(vs[m][h]), -126.0f);
+            lv[m][h] = fmaxf(log2_fast(vs[m][h]), S::LEAST_LOG);
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n)
