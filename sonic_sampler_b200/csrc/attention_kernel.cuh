@@ -779,7 +779,7 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
             const uint32_t at = stage + 2 * S::TILE + (m * 16 + 8 * h + g) * 4;
             ks *= __uint_as_float(load_shared4(at));
             vs[m][h] = __uint_as_float(load_shared4(at + KT * 4));
-            lv[m][h] = fmaxf(log2_fast(vs[m][h]), S::LEAST_LOG);
+            lv[m][h] = fmaxf(log2_fast(fabsf(vs[m][h])), S::LEAST_LOG);
           }
 #pragma unroll
           for (int n = 0; n < NT; ++n)

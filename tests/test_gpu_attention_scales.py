@@ -102,3 +102,13 @@ def test_scales_tiny_and_large(dev, power, way):  # noqa: F811
         for f in factors:
             f[::5] = 0.0
     _check(dev, lengths, [1] * len(lengths), 8, 2, 128, factors, seed=way, width=width)
+
+
+@pytest.mark.parametrize("way", range(len(WAYS)))
+def test_scales_of_either_sign(dev, way):  # noqa: F811
+    """A row stands for code * scale, whatever the scale's sign."""
+    lengths, width = WAYS[way]
+    factors = _ones(lengths, 2)
+    for f in factors:
+        f[::3] = -1.0
+    _check(dev, lengths, [1] * len(lengths), 8, 2, 128, factors, seed=way, width=width)
