@@ -816,12 +816,28 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
           rise = rise || v > ref[n][c] + S::SLACK;
         }
       if (__any_sync(ALL, rise)) {
+        // An infinite value scale makes the output so, and must leave the sum alone: it counts as 1. (Looked
+        // at here alone, where its key always leads: on every key's way it costs 1 % of a long call.)
+        if constexpr (Q8) {
+#pragma unroll
+          for (int m = 0; m < MK; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (lv[m][h] == INFINITY) lv[m][h] = 0.0f;
+        }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           float alpha[2];
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             float v = top[n][c];
+            if constexpr (Q8) {
+              v = -INFINITY;
+#pragma unroll
+              for (int m = 0; m < MK; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) v = fmaxf(v, s[m][n][2 * h + c] + lv[m][h]);
+            }
             v = fmaxf(v, __shfl_xor_sync(ALL, v, 4));
             v = fmaxf(v, __shfl_xor_sync(ALL, v, 8));
             v = fmaxf(v, __shfl_xor_sync(ALL, v, 16));

@@ -112,3 +112,26 @@ def test_scales_of_either_sign(dev, way):  # noqa: F811
     for f in factors:
         f[::3] = -1.0
     _check(dev, lengths, [1] * len(lengths), 8, 2, 128, factors, seed=way, width=width)
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("way", range(len(WAYS)))
+@pytest.mark.parametrize("at", [0, 20, -1])
+def test_log_sum_exps_do_not_depend_on_bad_value_scales(dev, bad, way, at):  # noqa: F811
+    """A value row that is not finite, the first, one of a later request's first keys or the newest: the
+    output is not finite where it is seen, the log-sum-exp is that of the keys."""
+    lengths, width = WAYS[way]
+    new = [2] * len(lengths)
+    factors = _ones(lengths, 2)
+    table, cache, held, q, first = _scaled(dev, lengths, new, 8, 2, 128, factors, way, width)
+    for b, n in enumerate(lengths):
+        p = at % n
+        cache.value_scales[table[b, p // 16].long(), :, p % 16] = bad
+    out, lse = _attend(dev, table, cache, q, lengths, new, first, 8, 2, 128)
+    expect, bound, expect_lse, lse_bound = _expect(q, held, lengths, new, first, 2)
+    assert ((lse.double() - expect_lse).abs() <= lse_bound).all()
+    for b, n in enumerate(lengths):
+        rows = slice(first[b] + (at == -1), first[b] + 2)
+        assert not torch.isfinite(out[rows]).any()
+        if at == -1:  # the request's first query does not see its last key
+            assert ((out[first[b]].double() - expect[first[b]]).abs() <= bound[first[b]]).all()
