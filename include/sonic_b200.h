@@ -423,9 +423,9 @@ typedef struct SonicPagedCache {
 /*
  * Which tokens a call is about. Request b has lengths[b] tokens in the cache, the call's new ones
  * included: these are its last n_b, rows [cu_seqlens[b], cu_seqlens[b + 1]) of the call's token
- * tensors (without cu_seqlens, tokens / requests rows each). The token at position t lies in page
- * page_table[b * table_stride + t / page_size], slot t % page_size. All arrays are read on the
- * device, so a captured graph follows them.
+ * tensors (without cu_seqlens, tokens / requests rows each). cu_seqlens must not decrease. The token
+ * at position t lies in page page_table[b * table_stride + t / page_size], slot t % page_size. All
+ * arrays are read on the device, so a captured graph follows them.
  */
 typedef struct SonicSequences {
   int32_t requests;
@@ -473,8 +473,9 @@ typedef struct SonicCacheGatherArgs {
 /* Attention of the call's tokens over their requests' cached keys and values, which already hold
  * the tokens themselves. Query i of request b stands at position lengths[b] - n_b + i and sees the
  * keys up to it, the last `window` of them when window > 0. out = sum_j softmax_j(scale q.k_j) v_j,
- * lse = log sum_j exp(scale q.k_j); a query that sees no key gives 0 and -infinity. What lies at
- * positions a query does not see never reaches its output, NaN and infinities included. */
+ * lse = log sum_j exp(scale q.k_j); a query that sees no key gives 0 and -infinity, and so do rows outside
+ * every request (before cu_seqlens[0], or from cu_seqlens[requests] on). What lies at positions a query
+ * does not see never reaches its output, NaN and infinities included. */
 typedef struct SonicPagedAttentionArgs {
   SonicPagedCache cache;
   SonicSequences sequences;

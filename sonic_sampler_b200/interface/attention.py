@@ -63,7 +63,8 @@ class PagedAttention:
 
         Returns the output (in `output` where that is given), and with `logsumexp` also the fp32
         `[tokens, q_heads]` logarithms of the softmax sums, with which outputs over disjoint key
-        ranges can be joined. A query that sees no key gives zeros and -infinity."""
+        ranges can be joined. A query that sees no key gives zeros and -infinity, and so do rows outside
+        every request (a padded call's, before `cu_seqlens[0]` or from `cu_seqlens[-1]` on)."""
         struct, device, scratchpad = cache.struct, cache.device, self.scratchpad
         if struct.kv_heads != self.kv_heads or struct.head_dim != self.head_dim:
             raise ValueError("the cache's kv_heads and head_dim must match `initialize`'s")
