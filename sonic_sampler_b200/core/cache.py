@@ -19,16 +19,18 @@ from torch import Tensor
 
 from sonic_sampler_b200 import _abi, ops
 from sonic_sampler_b200._abi import FLAG_PDL
+from sonic_sampler_b200.core.described import Described
 
 E4M3 = torch.float8_e4m3fn
 
 
 @dataclass(eq=False)
-class PagedCache:
+class PagedCache(Described):
     """Pages of keys and values, `[pages, kv_heads, page_size, head_dim]` in bf16, fp16 or
     float8_e4m3fn; with float8_e4m3fn one fp32 scale per (page, head, slot), and a row stands for
     code * scale. Any strides with a unit inner one, shared by keys and values, rows on 16-byte
-    boundaries."""
+    boundaries. The calls after an assignment to a field use the new tensor, which must fit the others:
+    pages of another form make another PagedCache."""
 
     keys: Tensor
     values: Tensor
@@ -36,15 +38,17 @@ class PagedCache:
     value_scales: Tensor | None = None
     pdl: bool = True
 
-    def __post_init__(self):
-        self.struct = ops.paged_cache_struct(self.keys, self.values, self.key_scales, self.value_scales)
-        self.device = self.keys.device
-        self.flags = FLAG_PDL if self.pdl else 0
+    def describe(self) -> None:
+        struct = ops.paged_cache_struct(self.keys, self.values, self.key_scales, self.value_scales)
+        device = self.keys.device
         # the device error word of append and gather
-        self.errors = ops.new_workspace(256, self.device)
+        errors = getattr(self, "errors", None)
+        self.errors = errors if errors is not None and errors.device == device else ops.new_workspace(256, device)
+        self.struct, self.device = struct, device
+        self.flags = FLAG_PDL if self.pdl else 0
         # what `_abi.load_calls()`'s functions take of it
-        self.address = ctypes.addressof(self.struct)
-        self.place = (self.address, self.device.index, self.flags, self.errors.data_ptr())
+        self.address = ctypes.addressof(struct)
+        self.place = (self.address, device.index, self.flags, self.errors.data_ptr())
 
     @classmethod
     def allocate(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,

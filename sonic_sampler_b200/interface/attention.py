@@ -16,11 +16,12 @@ from torch import Tensor
 from sonic_sampler_b200 import _abi, ops
 from sonic_sampler_b200._abi import FLAG_PDL
 from sonic_sampler_b200.core.cache import PagedCache
+from sonic_sampler_b200.core.described import Described
 from sonic_sampler_b200.interface.base import default_device
 
 
 @dataclass(eq=False)
-class PagedAttention:
+class PagedAttention(Described):
     q_heads: int
     kv_heads: int
     head_dim: int
@@ -29,7 +30,7 @@ class PagedAttention:
     # zero-filled workspace of the kernel; calls that overlap on the GPU need objects of their own
     scratchpad: Tensor
 
-    def __post_init__(self):
+    def describe(self) -> None:
         self.template = ops.paged_attention_template(self.q_heads, self.head_dim, FLAG_PDL if self.pdl else 0)
         self.address = ctypes.addressof(self.template)
 

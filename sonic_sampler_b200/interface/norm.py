@@ -14,12 +14,13 @@ from torch import Tensor
 
 from sonic_sampler_b200 import _abi, ops
 from sonic_sampler_b200._abi import FLAG_PDL
+from sonic_sampler_b200.core.described import Described
 
 E4M3 = torch.float8_e4m3fn
 
 
 @dataclass(eq=False)
-class ResidualNorm:
+class ResidualNorm(Described):
     """r = x + residual, y = r / sqrt(mean(r^2) + eps) * weight, in fp32.
 
     `dtype=torch.float8_e4m3fn` returns y's e4m3 codes, with an fp32 scale per row or per `group`
@@ -31,7 +32,7 @@ class ResidualNorm:
     group: int | None = None
     pdl: bool = True
 
-    def __post_init__(self):
+    def describe(self) -> None:
         if self.dtype not in (None, E4M3, self.weight.dtype):
             raise ValueError(f"`dtype` must be float8_e4m3fn or the weight's {self.weight.dtype}, got {self.dtype}")
         if self.group not in (None, 128) or (self.group and self.dtype != E4M3):
