@@ -19,8 +19,8 @@ from pathlib import Path
 PACKAGE_DIR = Path(__file__).resolve().parent
 CSRC = PACKAGE_DIR / "csrc"
 OUT = PACKAGE_DIR / "_lib" / "libsonic_b200.so"
-# diagnostic variant with per-phase timing stamps (python -m sonic_sampler_b200.phases)
 CALLS = CSRC / "calls.cpp"
+# diagnostic variant with per-phase timing stamps (python -m sonic_sampler_b200.phases)
 STAMPS_OUT = PACKAGE_DIR / "_lib" / "libsonic_b200_stamps.so"
 API = PACKAGE_DIR.parent / "include" / "sonic_b200.h"
 EXPORTS = CSRC / "exports.map"
@@ -72,10 +72,13 @@ def stale(out: Path = OUT, sources: list[Path] = SOURCES + HEADERS) -> bool:
 
 
 def calls_path() -> Path:
-    """The CPython module for the torch that is installed (its C++ classes differ between versions)."""
+    """The CPython module for the installed torch (its C++ classes differ between versions) and the running
+    interpreter (so does its C interface)."""
+    import sysconfig
+
     import torch
 
-    return PACKAGE_DIR / "_lib" / f"sonic_b200_calls_{torch.__version__}.so"
+    return PACKAGE_DIR / "_lib" / f"sonic_b200_calls_{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so"
 
 
 def calls_command() -> list[str]:
