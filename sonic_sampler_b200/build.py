@@ -65,10 +65,11 @@ def nvcc_path() -> str:
 
 
 def stale(out: Path = OUT, sources: list[Path] = SOURCES + HEADERS) -> bool:
+    """Whether `out` is missing, or older than a source or this file (whose flags it was built with)."""
     if not out.is_file():
         return True
     t = out.stat().st_mtime
-    return any(p.stat().st_mtime > t for p in sources)
+    return any(p.stat().st_mtime > t for p in (*sources, Path(__file__)))
 
 
 def calls_path() -> Path:
