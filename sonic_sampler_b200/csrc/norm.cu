@@ -22,6 +22,7 @@ namespace sonic {
 namespace {
 
 constexpr int MAX_WARPS = 32;
+constexpr int MAX_HIDDEN = 32768;
 
 template <typename T>
 __device__ __forceinline__ float to_float(T x) {
@@ -369,11 +370,16 @@ sonic_status run(const SonicResidualNormArgs& a, cudaStream_t stream) {
     if (width == 8) return go(norm_kernel<T, Q8, VEC, 1, 8>);
     if (width == 16) return go(norm_kernel<T, Q8, VEC, 1, 16>);
   }
+  // (the widest row of 16-bit values in 16-byte pieces has 4 items a lane, the others' 8)
+  constexpr int MOST = MAX_HIDDEN / PER_WARP / MAX_WARPS;
+  static_assert(MOST == 4 || MOST == 8, "the variants below");
+  if constexpr (MOST == 8) {
+    if (n == 8) return go(norm_kernel<T, Q8, VEC, 8, 32>);
+  }
   switch (n) {
     case 1: return go(norm_kernel<T, Q8, VEC, 1, 32>);
     case 2: return go(norm_kernel<T, Q8, VEC, 2, 32>);
-    case 4: return go(norm_kernel<T, Q8, VEC, 4, 32>);
-    default: return go(norm_kernel<T, Q8, VEC, 8, 32>);
+    default: return go(norm_kernel<T, Q8, VEC, 4, 32>);
   }
 }
 
@@ -398,7 +404,7 @@ extern "C" sonic_status sonic_residual_norm(const SonicResidualNormArgs* a, void
   if (!a) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "args must not be NULL");
   if (a->rows < 0) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "rows must not be negative");
   if (a->hidden < 1) return fail_with(SONIC_ERR_INVALID_ARGUMENT, "hidden must be positive");
-  if (a->hidden > 32768) return fail_with(SONIC_ERR_UNSUPPORTED, "hidden must be at most 32768");
+  if (a->hidden > MAX_HIDDEN) return fail_with(SONIC_ERR_UNSUPPORTED, "hidden must be at most 32768");
   if (a->dtype != SONIC_DTYPE_BF16 && a->dtype != SONIC_DTYPE_F16 && a->dtype != SONIC_DTYPE_F32)
     return fail_with(SONIC_ERR_INVALID_ARGUMENT, "dtype must be bf16, f16 or f32");
   if (a->out_dtype != a->dtype && a->out_dtype != SONIC_DTYPE_E4M3)
