@@ -255,7 +255,7 @@ Work work_of(int tokens, int heads, int lanes, int items) {
 // blockIdx.y: rounds of a token with more pieces than one CTA takes
 dim3 grid_of(const Work& w, int tokens, int lanes, int items) {
   const int pieces = w.run * w.per_token * lanes;
-  return dim3((tokens + w.run - 1) / w.run, (pieces + items * NT - 1) / (items * NT));
+  return dim3((unsigned)(((int64_t)tokens + w.run - 1) / w.run), (pieces + items * NT - 1) / (items * NT));
 }
 
 bool is_16bit(int dtype) { return dtype == SONIC_DTYPE_BF16 || dtype == SONIC_DTYPE_F16; }

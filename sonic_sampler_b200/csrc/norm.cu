@@ -363,7 +363,7 @@ sonic_status run(const SonicResidualNormArgs& a, cudaStream_t stream) {
   int width = 32;
   if (VEC && warps == 1 && a.hidden <= PER_WARP / 2) width = a.hidden <= PER_WARP / 4 ? 8 : 16;
   const int rows = warps > 1 ? 1 : width < 32 ? 128 / width : std::min(a.rows, 4);  // whole warps
-  const dim3 block(width * warps, rows), grid((a.rows + rows - 1) / rows);
+  const dim3 block(width * warps, rows), grid((unsigned)(((int64_t)a.rows + rows - 1) / rows));
   const bool pdl = a.flags & SONIC_FLAG_PDL;
   const auto go = [&](auto kernel) { return launch_status(launch_kernel(kernel, grid, block, 0, stream, pdl, 1, a)); };
   if constexpr (VEC) {

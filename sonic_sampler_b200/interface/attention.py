@@ -42,6 +42,8 @@ class PagedAttention(Described):
             raise ValueError(f"head_dim must be 64, 128 or 256, got {head_dim}")
         if lookahead < 0:
             raise ValueError(f"lookahead must not be negative, got {lookahead}")
+        if lookahead >= ops.INT32_MAX:
+            raise ValueError(f"lookahead must be below 2^31 - 1, got {lookahead}")
         return cls(q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, lookahead=lookahead, pdl=pdl,
                    scratchpad=ops.new_workspace(ops.paged_attention_workspace_bytes(), default_device()))
 

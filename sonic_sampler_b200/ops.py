@@ -46,6 +46,7 @@ _INDEX_DTYPES = {I32: DT_I32, I64: DT_I64}
 _FLOAT_DTYPES = {BF16: DT_BF16, F32: DT_F32}
 _ACTIVATION_DTYPES = {BF16: DT_BF16, F16: DT_F16}
 _CACHE_DTYPES = {BF16: DT_BF16, F16: DT_F16, E4M3: DT_E4M3}
+INT32_MAX = 2**31 - 1  # (a struct's field would take larger numbers modulo 2^32)
 _NORM_DTYPES = {BF16: DT_BF16, F16: DT_F16, F32: DT_F32}
 
 
@@ -496,6 +497,8 @@ def _sequences(a, tokens: int, page_table: Tensor, lengths: Tensor | None, cu_se
         raise ValueError("`page_table` must be int32 [requests, pages] with a unit inner stride")
     if page_table.device != device:
         raise ValueError(f"`page_table` must be on {device}")
+    if max(tokens, requests, width) > INT32_MAX:
+        raise ValueError("tokens, requests and pages of a request must be below 2^31")
     s = a.sequences
     s.requests = requests
     s.table_width = width
@@ -617,7 +620,7 @@ def paged_attention_args(template: PagedAttentionArgs, cache: PagedCacheStruct, 
     a.cache = cache
     a.dtype = _ACTIVATION_DTYPES[dtype]
     a.max_tokens = max_tokens
-    a.window = window
+    a.window = min(window, INT32_MAX)  # (no request is longer)
     if scale is not None:
         a.scale = scale
     a.queries = queries.data_ptr()
@@ -660,6 +663,8 @@ def residual_norm_args(template: ResidualNormArgs, x: Tensor, weight: Tensor, re
     if x.dtype != dtype or x.device != device:
         raise ValueError(f"`x` must have the weight's dtype and device, {dtype} on {device}")
     rows = x.size(0)
+    if rows > INT32_MAX:
+        raise ValueError(f"`x` must have less than 2^31 rows, got {rows}")
     a.rows = rows
     a.x_stride = _norm_rows(x, "x", rows, hidden, dtype, device)
     a.x = x.data_ptr()
