@@ -91,7 +91,8 @@ class PagedCache(Described):
         An e4m3 row is code * scale, rounded once to `dtype` (bf16 by default, or fp16); other caches
         keep their dtype. `keys` and `values` may give the outputs to write."""
         if dtype is None:
-            dtype = keys.dtype if keys is not None else torch.bfloat16 if self.keys.dtype == E4M3 else self.keys.dtype
+            given = values if keys is None else keys
+            dtype = given.dtype if given is not None else torch.bfloat16 if self.keys.dtype == E4M3 else self.keys.dtype
         if keys is None and values is None and (dtype == torch.bfloat16 or dtype == torch.float16):
             rows = _abi.load_calls().gather(*self.place, page_table, starts, total, dtype == torch.float16)
             if type(rows) is tuple:
