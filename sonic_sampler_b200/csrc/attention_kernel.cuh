@@ -6,9 +6,10 @@
 // m need not be the maximum: it is raised (and l and out rescaled) only when a score passes it by
 // 2^SLACK, so most tiles reduce nothing across lanes.
 //
-// Bound by memory: G = q_heads / kv_heads query heads share a key, so a cached byte meets 2 G n
-// multiply-adds (n new tokens), far below the tensor cores' balance. The work is laid out for a
-// continuous stream of the cache:
+// Bound by memory: G = q_heads / kv_heads query heads share a key, and each cached element takes part in one
+// multiply-add a query row, so a cached byte meets G n of them (n new tokens; e4m3) or G n / 2 (16 bits),
+// far below the tensor cores' balance of some 125 a byte. The work is laid out for a continuous stream
+// of the cache:
 // - A unit is (request, kv head, tile of up to 8 NT query rows). All units are laid end to end by
 //   their cost (their tiles of KT keys, and START for the unit itself) and cut into equal shares,
 //   one a warp, whatever the lengths: a warp finds its place with a scan over `lengths`, and streams
@@ -26,19 +27,24 @@
 //   are at least 64 rows by 128 lanes of tensor memory and would take their operands from shared
 //   memory, where e4m3 tiles would first have to be widened; these fragments widen in registers.
 // - An e4m3 key row is code * scale: the scale multiplies the score after the product. A value row's
-//   scale vs multiplies the softmax weight, and m follows u_j + log2 vs_j, so that the fp16 weights
-//   keep their precision whatever the scales. Codes become fp16 exactly; query rows are brought to
-//   fp16's range by a power of two.
+//   scale vs multiplies the softmax weight, and m follows u_j + log2 |vs_j|, so that the fp16 weights keep
+//   their precision from one value scale to another (below 2^-80 they fade). A weight times scale of less
+//   than 2^-24 of the leading one is fp16 subnormal: off by less than 2^-34 of the leading row's values.
+//   Codes become fp16 exactly; query rows are brought to fp16's range by a power of two.
 //
-// Measured (device time, head_dim 128, 4 query heads a kv head unless named): 128 requests of 2048 to
-// 16384 keys, e4m3 cache, one token each 302 us (6.2 TB/s of the cache's bytes); 64 requests of 1 to
-// 8192 keys, bf16, 52 us (5.0); 2 requests of 100003 and 131072 keys, 8 query heads, e4m3, 89 us (5.4);
-// one request of 700 keys 7.5 us: launch, one trip to memory and the join over the cluster. With many
-// query rows the products' latency bounds it, not the memory: two warps a scheduler hold all of its
+// Measured (device time of repeated calls, three caches in turn, head_dim 128, 4 query heads a kv head
+// unless named): 128 requests of 2048 to 16384 keys, e4m3 cache, one token each 303 us (6.2 TB/s of the
+// cache's bytes); 64 requests of 1 to 8192 keys, bf16, 52 us (5.0); 2 requests of 100003 and 131072 keys,
+// 8 query heads, e4m3, 89 us (5.4); one request of 700 keys 7.5 us: launch, one trip to memory and the
+// join over the cluster (13 us with a page table for 131072 tokens, which takes the equal shares). With
+// many query rows the products' latency bounds it, not the memory: two warps a scheduler hold all of its
 // registers, and a tile of 16 keys takes a warp some 3000 cycles at 24 rows, 1500 of them the matrix
-// instructions' of both warps. 32 requests of up to 4097 keys, 1 to 5 tokens, bf16, 27 us (2.4 TB/s);
-// 32 requests of 100 to 8192 keys, 4 tokens of 8 query heads, e4m3, 67 us (1.9). Skipping the column
-// tiles that a request's rows do not fill changes neither: the longest shares are full ones.
+// instructions' of both warps. 32 requests of up to 4097 keys, 1 to 5 tokens, bf16, 27.5 us (2.4 TB/s, from
+// L2 in part); 32 requests of 100 to 8192 keys, 4 tokens of 8 query heads, e4m3, 67 us (1.9). Skipping the
+// column tiles that a request's rows do not fill changes neither: the longest shares are full ones.
+// A unit's row tiles beyond those that the hint of new tokens foresees are taken one after the other, each
+// over all of the request's keys: one prompt of 2000 tokens takes 302 us with its own length as the hint,
+// 698 in equal shares with a hint of one token, and 8005 with a fixed number of warps and that hint.
 
 #pragma once
 
@@ -197,7 +203,7 @@ struct Shape {
   static constexpr int RECORD = ROWS * D * 4;  // a partial result
   static_assert(WARP_BYTES >= RECORD, "it fits the ring");
   static_assert(STAGE % 128 == 0 && WARP_BYTES % 128 == 0, "the permutations below work on addresses");
-  static constexpr int OCC = SMEM <= 108 * 1024 ? 2 : 1;  // (and 4 KB of static shared memory)
+  static constexpr int OCC = SMEM <= 108 * 1024 ? 2 : 1;  // (beside 5 KB of static shared memory)
   static constexpr int CTAS = 148 * OCC;
   static_assert(ROWS * D <= PART_FLOATS && ROWS <= PART_ROWS && STAGES < QUEUE, "sizes");
   // m is raised when a score passes it by 2^SLACK; weights of fp16 products lie 2^SHIFT higher, at
@@ -324,6 +330,10 @@ __global__ void __launch_bounds__(NT_THREADS, (Shape<A, Q8, D, NT>::OCC)) attent
   __shared__ uint32_t arrived_last;
   __shared__ alignas(8) float query_back[WARPS][PART_ROWS];
   __shared__ const char* row_address[WARPS][32];  // key rows of a tile that is copied row by row
+  constexpr size_t STATIC = sizeof(scan) + sizeof(place) + sizeof(queue) + sizeof(shared_piece) + sizeof(shared_live) + sizeof(ring_stats) +
+                            sizeof(cta_stats) + sizeof(arrived_last) + sizeof(query_back) + sizeof(row_address) + 128;
+  // (an SM has 228 KB, of which it keeps 1 for each CTA)
+  static_assert(S::OCC * (S::SMEM + STATIC + 1024) <= 228 * 1024, "OCC CTAs share an SM");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;  // fragment row, and pair of columns
   const SonicSequences& seq = p.a.sequences;

@@ -3,15 +3,17 @@
 //
 // Bound by memory: one pass, the row stays in registers between the sum of squares and the output.
 // A row belongs to one CTA, to one warp where a warp's registers hold it (short rows pay no block
-// barrier), or to the 8 or 16 lanes of a warp that it fills. Each lane holds N items of P values: P consecutive ones in a 16-byte piece
-// where rows are aligned, else 4 values 32 columns apart (a warp then still reads consecutive
-// addresses, and an item of a warp is 128 consecutive columns in both layouts of a group).
+// barrier), or to the 8 or 16 lanes of a warp that it fills. Each lane holds N items of P values: P
+// consecutive ones in a 16-byte piece where rows are aligned, else 4 values 32 columns apart (a warp then
+// still reads consecutive addresses, and an item of a warp is 128 consecutive columns in both layouts of
+// a group).
 //
-// bf16 with a residual to e4m3, device time: 16384 x 8192 138 us with a scale a row, 141 us a scale per
-// 128 columns (6.8 and 6.7 TB/s of the bytes that it has to move); 64 x 4096 2.7 us, launch and one
-// trip to memory. 32768 x 128, 16 lanes a row, 7.4 us (a warp a row: 12.0). The strided layout is bound
-// by instructions, some 30 a value: 3000 x 5001 takes 30 us, twice what its bytes would. With a
-// division and a maximum by bits for every 128 columns in every lane those were 141 -> 150 us and 31 -> 36.
+// bf16 with a residual to e4m3, device time in a captured graph: 16384 x 8192 138 us with a scale a row, 142 us
+// a scale per 128 columns (6.8 and 6.7 TB/s of the bytes that it has to move, above this card's measured copy
+// rate of 6.55; as calls one after the other 150 to 158 us); 64 x 4096 2.6 us, launch and one trip to memory.
+// 32768 x 128, 16 lanes a row, 7.4 us (a warp a row: 12.0). The strided layout is bound by instructions, some
+// 30 a value: 3000 x 5001 takes 30 us, twice what its bytes would. With a division and a maximum by bits for
+// every 128 columns in every lane, 16384 x 8192 by groups took 150 us for 141, 3000 x 5001 by groups 36 for 31.
 
 #include <algorithm>
 
