@@ -482,7 +482,8 @@ typedef struct SonicPagedAttentionArgs {
   uint32_t flags;            /* SONIC_FLAG_PDL */
   int32_t dtype;             /* of queries and out: bf16 or f16 (the cache's own unless it is e4m3) */
   int32_t q_heads;           /* a multiple of kv_heads; query head h reads kv head h / (q_heads / kv_heads) */
-  int32_t max_tokens;        /* most new tokens a request has, or 0 when unknown: picks a tile height */
+  int32_t max_tokens;        /* most new tokens a request has, or 0 when unknown (tokens / requests then):
+                              * lays out the work; with cu_seqlens a request may bring more, slowly */
   int32_t window;            /* keys a query sees at most, or 0 for all */
   float scale;
   const void* queries;       /* [tokens, q_heads, head_dim], unit inner stride */

@@ -62,7 +62,8 @@ class PagedAttention(Described):
         Rows `cu_seqlens[b]:cu_seqlens[b + 1]` (without it, tokens / requests rows each) are the
         last tokens of request b, which has `lengths[b]` in the cache. Each sees the keys up to its
         own position, the last `window` of them where that is given. `scale` is 1 / sqrt(head_dim)
-        by default. `lookahead` of `initialize` is a hint: requests may bring more tokens.
+        by default. `lookahead` of `initialize` is a hint: requests may bring more tokens with
+        `cu_seqlens`, but slowly (give prompts an object of their own).
 
         Returns the output (in `output` where that is given), and with `logsumexp` also the fp32
         `[tokens, q_heads]` logarithms of the softmax sums, with which outputs over disjoint key
